@@ -300,6 +300,91 @@ int rexsc_fxp_conv2d_fwd(const rexsc_fxp_conv_desc *desc, const void *d_act, con
                          int32_t *d_out, void *d_workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * Linear layers in 8-bit integers, with a scale for each row of either operand (token of the activations, output channel of
+ * the weights).  The digital counterpart of the SC linear op; no counterpart among the reference's ops, whose quantised
+ * linear layer is a torch loop over the bits of a stream (utils_functional.py:955-1082).
+ *
+ * A row with the largest magnitude a > 0 is held as scale = a / 127 (fp32) and whole numbers q = 127 x / a rounded to the
+ * nearest, ties to even, decided by the exact quotient.  A row of zeros has scale 0 and q = 0; a row that holds an infinity
+ * or a NaN has scale NaN and q = 0, so that its outputs are NaN and no other row's are.
+ *
+ *   y[m, n]  = (sum_k qx[m, k] qw[n, k]) * sx[m] * sw[n] + bias[n]
+ *   g[m, n]  = dy[m, n] * sw[n] (held in fp32), quantised by rows:     dx[m, k] = sg[m] * sum_n qg[m, n] qw[n, k]
+ *   h[m, n]  = dy[m, n] * sx[m] (held in fp32), quantised by columns:  dw[n, k] = sh[n] * sum_m qh[m, n] qx[m, k]
+ *   db[n]    = sum_m dy[m, n]
+ *
+ * Sums of products are exact (int32: contractions up to REXSC_INT8_MAX_DOT, beyond which calls return REXSC_E_TOO_LONG); the
+ * scales are applied in fp32 and the result is rounded once.  Quantised matrices live in a layout of the library's own
+ * (`d_data`, rexsc_int8_data_size bytes, 256-byte aligned); rexsc_int8_pack / _unpack convert from and to row-major int8.
+ *   d_x, d_dy     fp32 / fp16 / bf16 (REXSC_*), rows `row_stride` elements apart, elements of a row next to each other
+ *   d_out, d_dx, d_dw  dense; d_bias, d_db  [n]; each of its own REXSC_* type
+ * Extents are 1 to 2^30.  Any of d_dx, d_dw, d_db may be null; d_x (d_w) is needed for d_dw (d_dx) only.
+ * `kernel`: REXSC_INT8_AUTO, or one of the two product kernels; results are identical.
+ * rexsc_int8_status synchronises the stream and returns REXSC_E_DEVICE_TIMEOUT if a bounded device-side wait of an int8
+ * product on the current device gave up since it was last asked (that call's outputs are incomplete), else REXSC_OK.
+ */
+#define REXSC_INT8_MAX_DOT 131071
+enum { REXSC_INT8_AUTO = 0, REXSC_INT8_SPLIT = 1, REXSC_INT8_PAIR = 2 };
+size_t rexsc_int8_data_size(int64_t rows, int64_t cols);
+int rexsc_int8_quantize(const void *d_x, int32_t dtype, int64_t rows, int64_t cols, int64_t row_stride, int8_t *d_data,
+                        float *d_scale, void *stream);
+int rexsc_int8_pack(const int8_t *d_q, int64_t rows, int64_t cols, int64_t row_stride, int8_t *d_data, void *stream);
+int rexsc_int8_unpack(const int8_t *d_data, int64_t rows, int64_t cols, int8_t *d_q, void *stream);
+int rexsc_int8_matmul(const int8_t *d_a, const float *d_a_scale, const int8_t *d_b, const float *d_b_scale,
+                      const void *d_bias, int32_t bias_dtype, int64_t m, int64_t n, int64_t k, void *d_out,
+                      int32_t out_dtype, int32_t kernel, void *stream);
+size_t rexsc_int8_linear_workspace_size(int64_t m, int64_t k);
+int rexsc_int8_linear_fwd(const void *d_x, int32_t dtype, int64_t m, int64_t k, int64_t row_stride, const int8_t *d_w,
+                          const float *d_w_scale, int64_t n, const void *d_bias, int32_t bias_dtype, void *d_out,
+                          int32_t out_dtype, int32_t kernel, void *d_workspace, size_t workspace_bytes, void *stream);
+size_t rexsc_int8_linear_bwd_workspace_size(int64_t m, int64_t n, int32_t want_dx, int32_t want_dw, int32_t want_db);
+int rexsc_int8_linear_bwd(const void *d_dy, int32_t dtype, int64_t m, int64_t n, int64_t k, int64_t row_stride,
+                          const int8_t *d_x, const float *d_x_scale, const int8_t *d_w, const float *d_w_scale, void *d_dx,
+                          int32_t dx_dtype, void *d_dw, int32_t dw_dtype, void *d_db, int32_t db_dtype, int32_t kernel,
+                          void *d_workspace, size_t workspace_bytes, void *stream);
+int rexsc_int8_status(void *stream);
+
+/*
+ * One AdamW step over many tensors.  The reference's loops take torch's optimizers (main_imagenet.py:212-213,
+ * main_conv.py:232-233); no counterpart among its ops.
+ *
+ *   g' = g / grad_scale     m' = beta1 m + (1 - beta1) g'     v' = beta2 v + (1 - beta2) g'^2     t = steps so far + 1
+ *   p' = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
+ *
+ * in fp32, p' rounded once to the parameter's type.  Moments live in flat buffers made of blocks of 256 elements; a tensor
+ * takes ceil(numel / 256) blocks from first_block on (ascending, without overlap), in the order of its memory; what pads its
+ * last block is rewritten like the moments of an element whose gradient is 0, and other blocks are left as they are.
+ *   state_bits 32  d_exp_avg, d_exp_avg_sq: m and v as fp32
+ *   state_bits 8   d_exp_avg, d_exp_avg_sq: m and r = sqrt(v) as e4m3 bytes, times the block's fp32 in d_*_scale (largest
+ *                  magnitude / 448).  Cut to e4m3 and rounded up where the cut-off fraction of a step, in units of 2^-20,
+ *                  plus u >> 12 reaches 2^20; u = (place in the flat buffer * 0xC13FA9A9 + t * 0x9E3779B9) mod 2^32 for m
+ *                  and its complement for r: the mean over the steps is right where rounding to nearest would never move.
+ *                  r' > 0 is not stored as 0.  Blocks with no magnitude of 2^-100 or more are stored as 0.
+ *   d_step         int64[2]: steps so far, and a counter that is 0 between calls.  `advance`: this call is the last of a step
+ *                  (calls with other parameter types or hyperparameters may precede it on the stream) and adds 1 to it.
+ *   d_lr           fp32 on the device in place of `lr`, or null
+ *   d_grad_scale, d_found_inf  fp32 as a GradScaler has them, or null; found_inf != 0: nothing is changed, the count neither
+ * Everything but d_param, the moments and d_step is only read.  The list may be reused as soon as the call returns.
+ */
+typedef struct rexsc_adamw_tensor {
+    void *d_param;        /* dense, param_dtype */
+    const void *d_grad;   /* the same order of elements, grad_dtype */
+    int64_t numel;
+    int64_t first_block;
+} rexsc_adamw_tensor;
+typedef struct rexsc_adamw_desc {
+    int32_t param_dtype, grad_dtype;   /* REXSC_F32 / F16 / BF16 */
+    int32_t state_bits;                /* 32 or 8 */
+    int32_t advance;
+    double lr, beta1, beta2, eps, weight_decay;
+    const float *d_lr, *d_grad_scale, *d_found_inf;
+    int64_t *d_step;
+    void *d_exp_avg, *d_exp_avg_sq;    /* 32-byte aligned */
+    float *d_exp_avg_scale, *d_exp_avg_sq_scale;
+} rexsc_adamw_desc;
+int rexsc_adamw_step(const rexsc_adamw_desc *desc, const rexsc_adamw_tensor *tensors, int32_t count, void *stream);
+
+/*
  * Register-only LOP3 issue-rate probe used by the benchmark to measure the integer-ALU roofline the
  * SC conv kernels are measured against.  Launches `blocks` x 256 threads doing `iters` x 64 dependent-free
  * LOP3 per thread; d_sink receives one word per thread.  Total lane-ops = blocks*256*iters*64.

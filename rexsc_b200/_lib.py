@@ -14,6 +14,8 @@ ERRORS = {
     -5: "REXSC_E_CUDA", -6: "REXSC_E_DEVICE_TIMEOUT", -7: "REXSC_E_STATIC_SCRATCH",
 }
 F32, F16, BF16 = 0, 1, 2
+INT8_AUTO, INT8_SPLIT, INT8_PAIR = 0, 1, 2
+INT8_MAX_DOT = 131071
 KERNEL_AUTO, KERNEL_DIRECT, KERNEL_TILED, KERNEL_TENSOR = 0, 1, 2, 3
 
 
@@ -31,6 +33,19 @@ class FxpConvDesc(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "batch", "c_in", "h_in", "w_in", "c_out", "kh", "kw", "pad_h", "pad_w", "stride_h", "stride_w",
         "act_dtype", "w_dtype", "add_config", "precision_in", "precision_out", "kernel")]
+
+
+class AdamWTensor(C.Structure):
+    """Mirror of rexsc_adamw_tensor (include/rexsc_b200.h)."""
+    _fields_ = [("d_param", C.c_void_p), ("d_grad", C.c_void_p), ("numel", C.c_int64), ("first_block", C.c_int64)]
+
+
+class AdamWDesc(C.Structure):
+    """Mirror of rexsc_adamw_desc (include/rexsc_b200.h)."""
+    _fields_ = ([(n, C.c_int32) for n in ("param_dtype", "grad_dtype", "state_bits", "advance")]
+                + [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+                + [(n, C.c_void_p) for n in ("d_lr", "d_grad_scale", "d_found_inf", "d_step", "d_exp_avg", "d_exp_avg_sq",
+                                             "d_exp_avg_scale", "d_exp_avg_sq_scale")])
 
 
 # name -> (restype, argtypes); every symbol include/rexsc_b200.h declares
@@ -64,6 +79,19 @@ SYMBOLS = {
     "rexsc_sc_calib_windows": (C.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _vp, _vp]),
     "rexsc_fxp_conv2d_workspace_size": (_sz, [C.POINTER(FxpConvDesc)]),
     "rexsc_fxp_conv2d_fwd": (C.c_int, [C.POINTER(FxpConvDesc), _vp, _vp, _vp, _vp, _sz, _vp]),
+    "rexsc_int8_data_size": (_sz, [_i64, _i64]),
+    "rexsc_int8_quantize": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "rexsc_int8_pack": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp]),
+    "rexsc_int8_unpack": (C.c_int, [_vp, _i64, _i64, _vp, _vp]),
+    "rexsc_int8_matmul": (C.c_int, [_vp] * 5 + [_i32] + [_i64] * 3 + [_vp, _i32, _i32, _vp]),
+    "rexsc_int8_linear_workspace_size": (_sz, [_i64, _i64]),
+    "rexsc_int8_linear_fwd": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _i32, _vp, _sz,
+                                        _vp]),
+    "rexsc_int8_linear_bwd_workspace_size": (_sz, [_i64, _i64, _i32, _i32, _i32]),
+    "rexsc_int8_linear_bwd": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp,
+                                        _i32, _i32, _vp, _sz, _vp]),
+    "rexsc_int8_status": (C.c_int, [_vp]),
+    "rexsc_adamw_step": (C.c_int, [C.POINTER(AdamWDesc), _vp, _i32, _vp]),
     "rexsc_alu_probe": (C.c_int, [_i32, _i32, _vp, _vp]),
     "rexsc_mma_probe": (C.c_int, [_i32, _i32, _i32, _vp, _vp]),
 }

@@ -1,0 +1,57 @@
+// 8-bit matrices of the linear layers: their layout, and the quantisation of one value.
+//
+// Layout ("tiled"): an R x C matrix of int8 is cut into tiles of 128 rows x 128 columns, tile (i, j) at
+// (i * ceil(C / 128) + j) * 16 KiB.  Inside a tile, row r's 128 bytes lie at r * 128 and its 16-byte chunks are permuted,
+// chunk c at c ^ (r & 7): the 128-byte swizzle of the tensor core's shared-memory operands.  A tile is therefore one
+// contiguous copy, and the same image serves as an operand whose contraction runs along the columns (K-major: y = x w^T)
+// and as one whose contraction runs along the rows (MN-major: the gradients), without a transposed copy.
+// Columns that pad the last tile are zero; rows that pad it are zero where the matrix is a handle of the caller's.
+#pragma once
+
+#include "common.cuh"
+
+namespace rexsc {
+
+constexpr int kI8Tile = 128;                    // rows and columns of a tile
+constexpr int kI8TileBytes = kI8Tile * kI8Tile; // 16 KiB
+constexpr long long kI8MaxDot = REXSC_INT8_MAX_DOT; // sums of so many products of -128 .. 127 do not overflow int32
+static_assert(kI8MaxDot * 128 * 128 < (1ll << 31), "int32 sums");
+
+static inline long long i8_tiles(long long n) { return (n + kI8Tile - 1) / kI8Tile; }
+static inline size_t i8_bytes(long long rows, long long cols) { return (size_t)i8_tiles(rows) * i8_tiles(cols) * kI8TileBytes; }
+static inline size_t dtype_bytes(int dtype) { return dtype == REXSC_F32 ? 4 : 2; }
+
+// byte offset of column c (a multiple of 8 for 8-byte accesses) of row r; tcols = tiles per tile row
+__device__ __forceinline__ size_t i8_offset(long long r, long long c, long long tcols)
+{
+    return ((size_t)(r >> 7) * tcols + (size_t)(c >> 7)) * kI8TileBytes + (size_t)(r & 127) * 128 +
+           (size_t)(((((int)c >> 4) & 7) ^ ((int)r & 7)) << 4) + (size_t)(c & 15);
+}
+
+// ---- host launchers ------------------------------------------------------------------------------------------
+int launch_i8_quantize_rows(const void *d_x, int dtype, long long rows, long long cols, long long stride, int8_t *d_data,
+                            float *d_scale, bool pad_rows, cudaStream_t st);
+
+// out[i, j] = (sum_k a[i, k] b[j, k]) * row_scale[i] * col_scale[j] + bias[j]
+struct I8Operand {
+    const int8_t *data;
+    long long step_mn, step_k; // tiles from one 128-row block of the operand to the next, and from one 128-step of the
+                               // contraction to the next
+    long long mn_tiles;        // 128-row blocks that exist
+    int mn_major;              // 0: a tile's rows are the operand's rows; 1: a tile's rows are the contraction
+};
+struct I8Product {
+    I8Operand a, b;
+    long long m, n, k;      // rows and columns of the output, length of the contraction
+    const float *row_scale; // [m]
+    const float *col_scale; // [n] or null
+    const void *bias;       // [n] or null
+    int bias_dtype;
+    void *out;
+    int out_dtype;
+    long long out_stride;   // elements between rows of the output
+};
+// kernel: REXSC_INT8_*.  after_quantize: the launch may begin while the previous one on the stream (which writes operand a) still runs
+int launch_i8_product(const I8Product &p, int kernel, bool after_quantize, cudaStream_t st);
+
+} // namespace rexsc

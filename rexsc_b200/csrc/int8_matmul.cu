@@ -1,0 +1,670 @@
+// Products of 8-bit matrices with scales per row and per column, on the 5th-generation tensor cores:
+//   out[i, j] = (sum_k a[i, k] b[j, k]) * row_scale[i] * col_scale[j] + bias[j],
+// the sum exact in int32 (tcgen05.mma.kind::i8, accumulators in TMEM), the rest in fp32, rounded once to the output's type.
+// Operands are tiled and swizzled in memory (int8.cuh), so a pipeline stage is one or two contiguous bulk copies of at most
+// 16 KiB, needs no tensor map, and a matrix serves K-major or MN-major by a bit of the instruction descriptor.
+//
+// Two kernels:
+//   product_pair_kernel  pairs of CTAs (cta_group::2) on 256 x 256 output tiles, persistent, two accumulators per CTA so that
+//                        the epilogue of a tile runs under the next one's products.
+//   product_split_kernel 128 columns of the output (lanes of TMEM) x 16 to 128 rows per CTA; the CTAs of a cluster split the
+//                        contraction and join their int32 sums through distributed shared memory (whole numbers: the
+//                        order does not matter).
+// Every mbarrier wait is bounded; a CTA whose wait gives up raises the library's status word (rexsc_int8_status), stores
+// nothing more, waits for its copies in flight, frees its TMEM and leaves.
+#include "int8.cuh"
+
+namespace rexsc {
+
+namespace {
+
+__device__ int g_i8_status = 0; // != 0: a bounded wait gave up since rexsc_int8_status was last asked
+
+constexpr uint32_t kWaitLimit = 1u << 22;
+
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+// (acquire at cluster scope: some arrivals come from the other CTA of a pair)
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity)
+{
+    for (uint32_t i = 0; i < kWaitLimit; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    atomicExch(&g_i8_status, 1);
+    return false;
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank)
+{
+    uint32_t out;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
+    return out;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t mapped)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapped) : "memory");
+}
+__device__ __forceinline__ void copy_in(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void wait_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Shared-memory matrix descriptor, 128-byte swizzle.  Both ways of reading a tile share it: rows 128 bytes apart in groups of
+// 8 that are 1024 bytes apart.  K-major the rows are the operand's rows and 32 products are 32 bytes further; MN-major the
+// rows are the contraction and 32 products are 32 rows (4096 bytes) further.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr)
+{
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3fff);
+    d |= (uint64_t)(kI8TileBytes >> 4) << 16; // next 128 along MN (not reached: one tile is as wide)
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// instruction descriptor: int32 sums, signed 8-bit operands, their major-ness, M and N
+__host__ __device__ __forceinline__ uint32_t product_idesc(int m, int n, int a_mn, int b_mn)
+{
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_load32(uint32_t addr, int (&v)[32])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, int *v)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// ---- output values --------------------------------------------------------------------------------------------
+__device__ __forceinline__ float load_any(const void *p, int dtype, long long i)
+{
+    if (dtype == REXSC_F32) return static_cast<const float *>(p)[i];
+    if (dtype == REXSC_F16) return __half2float(static_cast<const __half *>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+template <typename T> __device__ __forceinline__ T round_to(float v);
+template <> __device__ __forceinline__ float round_to<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ uint32_t pack2(__half a, __half b)
+{
+    return (uint32_t)__half_as_ushort(a) | (uint32_t)__half_as_ushort(b) << 16;
+}
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b)
+{
+    return (uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16;
+}
+__device__ __forceinline__ float scaled(int sum, float row, float col, float bias)
+{
+    return fmaf(__fmul_rn(__int2float_rn(sum), row), col, bias);
+}
+
+struct PairArgs {
+    I8Product p;
+    long long tiles_i, tiles_j; // 256 x 256 output tiles
+    int k_blocks;
+    int store_bytes;            // bytes that every row of the output is aligned to: 32, 16, or fewer
+};
+
+constexpr int kPairStages = 6;
+constexpr int kPairStageBytes = 2 * kI8TileBytes;
+constexpr int kPairThreads = 192;     // producer, products, four warps for the epilogue
+constexpr int kGroupTiles = 8;        // output tile rows that share the columns' operand while it is in L2
+constexpr size_t kPairSmem = kPairStages * kPairStageBytes + 1024 + 2 * 256 * 2 * sizeof(float) + 256;
+
+// one lane's 32 neighbouring columns of a row
+template <typename T>
+__device__ __forceinline__ void store_row(T *dst, const float (&v)[32], int live, int store_bytes)
+{
+    if (live >= 32 && store_bytes >= 16) {
+        if constexpr (sizeof(T) == 4) {
+            if (store_bytes >= 32) {
+#pragma unroll
+                for (int i = 0; i < 32; i += 8)
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + i), "f"(v[i]),
+                                 "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]),
+                                 "f"(v[i + 7]) : "memory");
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                    *reinterpret_cast<float4 *>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+            }
+        } else {
+            uint32_t w[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) w[i] = pack2(round_to<T>(v[2 * i]), round_to<T>(v[2 * i + 1]));
+            if (store_bytes >= 32) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 8)
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 2 * i), "r"(w[i]),
+                                 "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]),
+                                 "r"(w[i + 7]) : "memory");
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                    *reinterpret_cast<uint4 *>(dst + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; i++)
+            if (i < live) dst[i] = round_to<T>(v[i]);
+    }
+}
+
+// Output tile t of the persistent schedule: groups of kGroupTiles tile rows, column by column.
+__device__ __forceinline__ void tile_of(long long t, const PairArgs &a, long long *ti, long long *tj)
+{
+    const long long per_group = kGroupTiles * a.tiles_j, g = t / per_group, rest = t - g * per_group;
+    const long long left = a.tiles_i - g * kGroupTiles, rows = left < kGroupTiles ? left : kGroupTiles;
+    *tj = rest / rows;
+    *ti = g * kGroupTiles + (rest - *tj * rows);
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+product_pair_kernel(const __grid_constant__ PairArgs a)
+{
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    float *col_s = reinterpret_cast<float *>(smem + kPairStages * kPairStageBytes); // [buffer][scale, bias][256]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(col_s + 2 * 2 * 256);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kPairStages + 5);
+    const uint32_t bar0 = smem_addr(bars);
+    auto full = [&](int s) { return bar0 + s * 8; };
+    auto empty = [&](int s) { return bar0 + (kPairStages + s) * 8; };
+    auto acc_full = [&](int b) { return bar0 + (2 * kPairStages + b) * 8; };
+    auto acc_empty = [&](int b) { return bar0 + (2 * kPairStages + 2 + b) * 8; };
+    const uint32_t drained = bar0 + (2 * kPairStages + 4) * 8;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const long long first = blockIdx.x >> 1, step = gridDim.x >> 1, tiles = a.tiles_i * a.tiles_j;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; s++) {
+            mbar_init(full(s), rank == 0 ? 2 : 1); // the leader's: its own copies and the word that the other's have landed
+            mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; b++) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), 8); // four warps of each CTA
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    wait_previous_launch();
+
+    if (warp == 0) {
+        if (lane == 0) { // ---- copies
+            uint32_t it = 0;
+            bool ok = true;
+            for (long long t = first; t < tiles && ok; t += step) {
+                long long ti, tj;
+                tile_of(t, a, &ti, &tj);
+                // a block behind the last one is read in its place: its sums are not stored
+                long long ia = ti * 2 + rank, ib = tj * 2 + rank;
+                ia = ia < a.p.a.mn_tiles ? ia : a.p.a.mn_tiles - 1;
+                ib = ib < a.p.b.mn_tiles ? ib : a.p.b.mn_tiles - 1;
+                const int8_t *pa = a.p.a.data + (size_t)(ia * a.p.a.step_mn) * kI8TileBytes;
+                const int8_t *pb = a.p.b.data + (size_t)(ib * a.p.b.step_mn) * kI8TileBytes;
+                for (int k = 0; k < a.k_blocks; k++, it++) {
+                    const int s = it % kPairStages;
+                    if (it >= kPairStages && !(ok = mbar_wait(empty(s), (it / kPairStages - 1) & 1))) break;
+                    const uint32_t dst = smem_addr(smem) + s * kPairStageBytes;
+                    mbar_expect(full(s), kPairStageBytes);
+                    copy_in(dst, pa + (size_t)(k * a.p.a.step_k) * kI8TileBytes, kI8TileBytes, full(s));
+                    copy_in(dst + kI8TileBytes, pb + (size_t)(k * a.p.b.step_k) * kI8TileBytes, kI8TileBytes, full(s));
+                }
+            }
+            // nothing on its way when this CTA leaves (at once, unless a wait gave up somewhere)
+            for (uint32_t j = it < kPairStages ? 0 : it - kPairStages; j < it; j++) mbar_wait(full(j % kPairStages), (j / kPairStages) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 1) { // ---- tell the leader that this CTA's copies have landed
+            uint32_t it = 0;
+            bool ok = true;
+            for (long long t = first; t < tiles && ok; t += step)
+                for (int k = 0; k < a.k_blocks; k++, it++) {
+                    const int s = it % kPairStages;
+                    if (!(ok = mbar_wait(full(s), (it / kPairStages) & 1))) break;
+                    mbar_arrive_cluster(map_rank(full(s), 0));
+                }
+        } else if (lane == 0) { // ---- products
+            const uint32_t idesc = product_idesc(256, 256, a.p.a.mn_major, a.p.b.mn_major);
+            const uint32_t adv_a = a.p.a.mn_major ? 4096 >> 4 : 32 >> 4, adv_b = a.p.b.mn_major ? 4096 >> 4 : 32 >> 4;
+            uint32_t it = 0;
+            int turn = 0;
+            bool ok = true;
+            for (long long t = first; t < tiles && ok; t += step, turn++) {
+                const int b = turn & 1;
+                if (turn >= 2 && !(ok = mbar_wait(acc_empty(b), (turn / 2 - 1) & 1))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int k = 0; k < a.k_blocks; k++, it++) {
+                    const int s = it % kPairStages;
+                    if (!(ok = mbar_wait(full(s), (it / kPairStages) & 1))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t sa = smem_addr(smem) + s * kPairStageBytes;
+                    const uint64_t da = tile_desc(sa), db = tile_desc(sa + kI8TileBytes);
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        asm volatile(
+                            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + b * 256),
+                            "l"(da + q * adv_a), "l"(db + q * adv_b), "r"(idesc), "r"((uint32_t)(k | q)) : "memory");
+                    asm volatile(
+                        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                            empty(s)), "h"((uint16_t)3) : "memory");
+                }
+                if (ok)
+                    asm volatile(
+                        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                            acc_full(b)), "h"((uint16_t)3) : "memory");
+            }
+            if (!ok) { // products in flight read both CTAs' stages and write their accumulators
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drained) : "memory");
+                mbar_wait(drained, 0);
+            }
+        }
+    } else { // ---- epilogue: a lane per row of this CTA's 128
+        const int quad = warp & 3, et = threadIdx.x - 64;
+        const uint32_t leader_empty = map_rank(acc_empty(0), 0);
+        T *out = static_cast<T *>(a.p.out);
+        int turn = 0;
+        for (long long t = first; t < tiles; t += step, turn++) {
+            const int b = turn & 1;
+            long long ti, tj;
+            tile_of(t, a, &ti, &tj);
+            const long long row = ti * 256 + rank * 128 + quad * 32 + lane, col0 = tj * 256;
+            float *cs = col_s + b * 512;
+            for (int i = et; i < 256; i += 128) {
+                const bool live = col0 + i < a.p.n;
+                cs[i] = live && a.p.col_scale ? a.p.col_scale[col0 + i] : 1.f;
+                cs[256 + i] = live && a.p.bias ? load_any(a.p.bias, a.p.bias_dtype, col0 + i) : 0.f;
+            }
+            const float rs = row < a.p.m ? a.p.row_scale[row] : 0.f;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (!mbar_wait(acc_full(b), (turn / 2) & 1)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+            for (int c = 0; c < 256; c += 32) {
+                if (col0 + c >= a.p.n) break; // (the same for all lanes)
+                __syncwarp();
+                int v[32];
+                tmem_load32(tmem + ((uint32_t)(quad * 32) << 16) + b * 256 + c, v);
+                float f[32];
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    const float4 s4 = *reinterpret_cast<const float4 *>(cs + c + i), b4 = *reinterpret_cast<const float4 *>(cs + 256 + c + i);
+                    f[i] = scaled(v[i], rs, s4.x, b4.x), f[i + 1] = scaled(v[i + 1], rs, s4.y, b4.y);
+                    f[i + 2] = scaled(v[i + 2], rs, s4.z, b4.z), f[i + 3] = scaled(v[i + 3], rs, s4.w, b4.w);
+                }
+                if (row < a.p.m) {
+                    const long long left = a.p.n - (col0 + c);
+                    store_row(out + row * a.p.out_stride + col0 + c, f, left < 32 ? (int)left : 32, a.store_bytes);
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(leader_empty + b * 8);
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+struct SplitArgs {
+    I8Product p;
+    long long tiles_j;  // blocks of 128 output columns
+    int rows;           // output rows per CTA: 16, 32, 64 or 128
+    int split;          // CTAs of the cluster
+    int k_blocks;
+    int stages;
+    int q_bytes;        // bytes of a stage's rows operand
+    int tmem_cols;
+    int store_bytes;
+};
+
+constexpr int kSplitThreads = 128;
+constexpr int kSplitMaxStages = 12;
+constexpr size_t kSplitSmemMost = 212 * 1024;
+
+template <typename T>
+__device__ __forceinline__ void store4(T *dst, const float (&v)[4], int live, bool aligned)
+{
+    if (live >= 4 && aligned) {
+        if constexpr (sizeof(T) == 4)
+            *reinterpret_cast<float4 *>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+        else
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(round_to<T>(v[0]), round_to<T>(v[1])), pack2(round_to<T>(v[2]), round_to<T>(v[3])));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i < live) dst[i] = round_to<T>(v[i]);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSplitThreads)
+product_split_kernel(const __grid_constant__ SplitArgs a)
+{
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * kSplitMaxStages + 1];
+    __shared__ uint32_t tmem_slot;
+    uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    const uint32_t bar0 = smem_addr(bars);
+    auto full = [&](int s) { return bar0 + s * 8; };
+    auto empty = [&](int s) { return bar0 + (kSplitMaxStages + s) * 8; };
+    const uint32_t acc_full = bar0 + 2 * kSplitMaxStages * 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = a.split > 1 ? (int)cluster_rank() : 0;
+    const long long tile = blockIdx.x / a.split, tj = tile % a.tiles_j, ti = tile / a.tiles_j;
+    const int k0 = (int)((long long)rank * a.k_blocks / a.split), k1 = (int)((long long)(rank + 1) * a.k_blocks / a.split);
+    const long long row0 = ti * a.rows, col0 = tj * 128;
+    const int rows = a.p.m - row0 < a.rows ? (int)(a.p.m - row0) : a.rows; // that exist
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < a.stages; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+        mbar_init(acc_full, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"((uint32_t)a.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    const uint32_t stage_bytes = kI8TileBytes + a.q_bytes;
+
+    if (warp == 0) {
+        if (lane == 0) { // ---- copies
+            const int8_t *pw = a.p.b.data + (size_t)(tj * a.p.b.step_mn) * kI8TileBytes;
+            const int8_t *px = a.p.a.data + (size_t)((row0 >> 7) * a.p.a.step_mn) * kI8TileBytes + (a.p.a.mn_major ? 0 : (row0 & 127) * 128);
+            const int n = k1 - k0, early = n < a.stages ? n : a.stages;
+            auto copy_w = [&](int i) {
+                const int s = i % a.stages;
+                mbar_expect(full(s), stage_bytes);
+                copy_in(smem_addr(smem) + s * stage_bytes, pw + (size_t)((k0 + i) * a.p.b.step_k) * kI8TileBytes, kI8TileBytes, full(s));
+            };
+            auto copy_x = [&](int i) {
+                const int s = i % a.stages;
+                copy_in(smem_addr(smem) + s * stage_bytes + kI8TileBytes, px + (size_t)((k0 + i) * a.p.a.step_k) * kI8TileBytes, a.q_bytes, full(s));
+            };
+            // the weights do not depend on the launch before, which quantises the rows
+            for (int i = 0; i < early; i++) copy_w(i);
+            wait_previous_launch();
+            for (int i = 0; i < early; i++) copy_x(i);
+            int i = early;
+            for (; i < n; i++) {
+                if (!mbar_wait(empty(i % a.stages), (i / a.stages - 1) & 1)) break;
+                copy_w(i);
+                copy_x(i);
+            }
+            for (int j = i < a.stages ? 0 : i - a.stages; j < i; j++) mbar_wait(full(j % a.stages), (j / a.stages) & 1);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) { // ---- products: lanes are output columns, columns of TMEM output rows
+            const uint32_t idesc = product_idesc(128, a.rows, a.p.b.mn_major, a.p.a.mn_major);
+            const uint32_t adv_w = a.p.b.mn_major ? 4096 >> 4 : 32 >> 4, adv_x = a.p.a.mn_major ? 4096 >> 4 : 32 >> 4;
+            for (int i = 0; i < k1 - k0; i++) {
+                const int s = i % a.stages;
+                if (!mbar_wait(full(s), (i / a.stages) & 1)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t sa = smem_addr(smem) + s * stage_bytes;
+                const uint64_t dw = tile_desc(sa), dx = tile_desc(sa + kI8TileBytes);
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    asm volatile(
+                        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+                        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+                        "l"(dw + q * adv_w), "l"(dx + q * adv_x), "r"(idesc), "r"((uint32_t)(i | q)) : "memory");
+                asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(empty(s)) : "memory");
+            }
+            // (after a wait that gave up: of what was issued)
+            asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(acc_full) : "memory");
+        }
+    }
+    __syncwarp();
+    wait_previous_launch();
+    mbar_wait(acc_full, 0);
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    T *out = static_cast<T *>(a.p.out);
+    const uint32_t tmem_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    auto free_tmem = [&]() {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncthreads();
+        if (warp == 1) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)a.tmem_cols) : "memory");
+        }
+    };
+    if (a.split == 1) {
+        const long long col = col0 + warp * 32 + lane;
+        const bool live = col < a.p.n;
+        const float cs = live && a.p.col_scale ? a.p.col_scale[col] : 1.f;
+        const float bias = live && a.p.bias ? load_any(a.p.bias, a.p.bias_dtype, col) : 0.f;
+        for (int c = 0; c < rows; c += 16) {
+            int v[16];
+            __syncwarp();
+            tmem_load16(tmem_lane + c, v);
+            if (live) {
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (c + i < rows)
+                        out[(row0 + c + i) * a.p.out_stride + col] = round_to<T>(scaled(v[i], a.p.row_scale[row0 + c + i], cs, bias));
+            }
+        }
+        __syncwarp();
+    } else {
+        // sums to shared memory, [row][column]; every CTA of the cluster finishes some of the rows
+        int *red = reinterpret_cast<int *>(smem);
+        for (int c = 0; c < rows; c += 16) {
+            int v[16];
+            tmem_load16(tmem_lane + c, v);
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (c + i < rows) red[(c + i) * 128 + warp * 32 + lane] = v[i];
+        }
+        // TMEM is given back before the CTAs of the cluster wait for one another: a CTA that holds TMEM then waits for nobody
+        // but itself, and one that waits for TMEM (of whatever kernel shares the SM) always gets it
+        free_tmem();
+        cluster_sync();
+        const long long col = col0 + lane * 4;
+        const int live = a.p.n - col < 4 ? (int)(a.p.n - col) : 4;
+        if (live > 0) {
+            float cs[4], bias[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                cs[i] = i < live && a.p.col_scale ? a.p.col_scale[col + i] : 1.f;
+                bias[i] = i < live && a.p.bias ? load_any(a.p.bias, a.p.bias_dtype, col + i) : 0.f;
+            }
+            for (int c = rank * 4 + warp; c < rows; c += 4 * a.split) {
+                int4 sum = make_int4(0, 0, 0, 0);
+                const uint32_t at = smem_addr(red + c * 128 + lane * 4);
+                for (int r = 0; r < a.split; r++) {
+                    int4 v;
+                    asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(map_rank(at, r)) : "memory");
+                    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+                }
+                const float rs = a.p.row_scale[row0 + c];
+                const float f[4] = {scaled(sum.x, rs, cs[0], bias[0]), scaled(sum.y, rs, cs[1], bias[1]),
+                                    scaled(sum.z, rs, cs[2], bias[2]), scaled(sum.w, rs, cs[3], bias[3])};
+                store4(out + (row0 + c) * a.p.out_stride + col, f, live, a.store_bytes >= 16);
+            }
+        }
+        __syncwarp();
+        cluster_sync(); // the others still read this CTA's sums
+    }
+    if (a.split == 1) free_tmem();
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------
+int store_alignment(const I8Product &p)
+{
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(p.out) | (uintptr_t)(p.out_stride * (long long)dtype_bytes(p.out_dtype));
+    return bits & 15 ? 0 : bits & 31 ? 16 : 32;
+}
+
+template <typename Args>
+int launch_cluster(void (*kernel)(Args), const Args &args, long long blocks, int cluster, int threads, size_t smem, bool overlap,
+                   cudaStream_t st, const char *name)
+{
+    if (blocks > 0x7fffffffll) return REXSC_E_UNSUPPORTED;
+    REXSC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = (unsigned)cluster;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        n++;
+    }
+    if (overlap) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        n++;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = (unsigned)n;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+    note_kernel_launch();
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        set_cuda_error(e, name);
+        return REXSC_E_CUDA;
+    }
+    return REXSC_OK;
+}
+
+template <typename T>
+int launch_pair(const I8Product &p, bool overlap, cudaStream_t st)
+{
+    PairArgs a;
+    a.p = p;
+    a.tiles_i = (p.m + 255) / 256;
+    a.tiles_j = (p.n + 255) / 256;
+    a.k_blocks = (int)i8_tiles(p.k);
+    a.store_bytes = store_alignment(p);
+    const long long tiles = a.tiles_i * a.tiles_j, pairs = tiles < 74 ? tiles : 74;
+    return launch_cluster(product_pair_kernel<T>, a, pairs * 2, 0, kPairThreads, kPairSmem, overlap, st, "product_pair_kernel");
+}
+
+template <typename T>
+int launch_split(const I8Product &p, bool overlap, cudaStream_t st)
+{
+    SplitArgs a;
+    a.p = p;
+    a.tiles_j = (p.n + 127) / 128;
+    a.k_blocks = (int)i8_tiles(p.k);
+    a.rows = p.a.mn_major || p.m > 64 ? 128 : p.m > 32 ? 64 : p.m > 16 ? 32 : 16;
+    const long long tiles = a.tiles_j * ((p.m + a.rows - 1) / a.rows);
+    a.split = 1;
+    while (a.split < 8 && a.split * 2 <= a.k_blocks && tiles * a.split * 2 <= 296) a.split *= 2;
+    a.q_bytes = p.a.mn_major ? kI8TileBytes : a.rows * 128;
+    const int stage = kI8TileBytes + a.q_bytes, most = (int)(kSplitSmemMost - 1024) / stage;
+    const int steps = (a.k_blocks + a.split - 1) / a.split;
+    a.stages = steps < kSplitMaxStages ? steps : kSplitMaxStages;
+    if (a.stages > most) a.stages = most;
+    a.tmem_cols = a.rows < 32 ? 32 : a.rows;
+    a.store_bytes = store_alignment(p);
+    size_t smem = (size_t)a.stages * stage;
+    if (a.split > 1 && smem < (size_t)a.rows * 512) smem = (size_t)a.rows * 512;
+    return launch_cluster(product_split_kernel<T>, a, tiles * a.split, a.split, kSplitThreads, smem + 1024, overlap, st,
+                          "product_split_kernel");
+}
+
+template <typename T>
+int launch_product(const I8Product &p, int kernel, bool overlap, cudaStream_t st)
+{
+    const long long tiles = ((p.m + 255) / 256) * ((p.n + 255) / 256);
+    const bool pair = kernel == REXSC_INT8_PAIR || (kernel == REXSC_INT8_AUTO && p.m > 128 && tiles >= 37);
+    return pair ? launch_pair<T>(p, overlap, st) : launch_split<T>(p, overlap, st);
+}
+
+} // namespace
+
+int launch_i8_product(const I8Product &p, int kernel, bool after_quantize, cudaStream_t st)
+{
+    switch (p.out_dtype) {
+    case REXSC_F32: return launch_product<float>(p, kernel, after_quantize, st);
+    case REXSC_F16: return launch_product<__half>(p, kernel, after_quantize, st);
+    default: return launch_product<__nv_bfloat16>(p, kernel, after_quantize, st);
+    }
+}
+
+} // namespace rexsc
+
+extern "C" int rexsc_int8_status(void *stream)
+{
+    using namespace rexsc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int seen = 0;
+    const int none = 0;
+    REXSC_CUDA_CHECK(cudaMemcpyFromSymbolAsync(&seen, g_i8_status, sizeof(seen), 0, cudaMemcpyDeviceToHost, st));
+    REXSC_CUDA_CHECK(cudaStreamSynchronize(st));
+    if (seen) REXSC_CUDA_CHECK(cudaMemcpyToSymbolAsync(g_i8_status, &none, sizeof(none), 0, cudaMemcpyHostToDevice, st));
+    return seen ? REXSC_E_DEVICE_TIMEOUT : REXSC_OK;
+}

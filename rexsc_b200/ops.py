@@ -674,6 +674,260 @@ def conv2d_saturate_acc(input: torch.Tensor, weight: torch.Tensor, add_config: i
     return out
 
 
+# ---- linear layers in 8-bit integers ----------------------------------------------------------------------
+def set_int8_kernel(name: str) -> None:
+    """Force the product kernel of the int8 ops: "auto", "split" or "pair"; results are identical, only speed differs."""
+    _kernel_choice.int8 = {"auto": _lib.INT8_AUTO, "split": _lib.INT8_SPLIT, "pair": _lib.INT8_PAIR}[name]
+
+
+def _int8_kernel() -> int:
+    return getattr(_kernel_choice, "int8", _lib.INT8_AUTO)
+
+
+class Int8Matrix:
+    """A matrix in 8-bit integers with an fp32 scale per row, as :func:`int8_quantize` makes it: row r stands for
+    ``values()[r] * scale[r]``.  ``data`` holds the integers in the library's own layout; keep the object as the prepared
+    weights of a layer and build a new one after the weights change."""
+
+    __slots__ = ("rows", "cols", "data", "scale")
+
+    def __init__(self, rows: int, cols: int, data: torch.Tensor, scale: torch.Tensor):
+        self.rows, self.cols, self.data, self.scale = rows, cols, data, scale
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.rows, self.cols
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+    @classmethod
+    def from_values(cls, values: torch.Tensor, scale: torch.Tensor) -> "Int8Matrix":
+        """From int8 ``values`` [rows, cols] and their ``scale`` [rows]."""
+        _require_cuda(values, "Int8Matrix.from_values")
+        if values.dtype != torch.int8 or values.dim() != 2 or 0 in values.shape:
+            raise ValueError("Int8Matrix.from_values: expected int8 values [rows, cols], neither of them 0")
+        rows, cols = values.shape
+        if scale.device != values.device or tuple(scale.shape) != (rows,) or not scale.is_floating_point():
+            raise ValueError("Int8Matrix.from_values: expected one scale per row on the values' device")
+        dev = values.device
+        with _on(dev):
+            v = values if values.stride(1) == 1 or cols == 1 else values.contiguous()
+            data = _int8_data(rows, cols, dev, "Int8Matrix.from_values")
+            _lib.check(_lib.load().rexsc_int8_pack(_ptr(v), rows, cols, v.stride(0), _ptr(data), _stream(dev)),
+                       "rexsc_int8_pack")
+            return cls(rows, cols, data, scale.detach().to(torch.float32, copy=True).contiguous())
+
+    def values(self) -> torch.Tensor:
+        """The integers, int8 [rows, cols]."""
+        dev = self.data.device
+        with _on(dev):
+            out = torch.empty((self.rows, self.cols), dtype=torch.int8, device=dev)
+            _lib.check(_lib.load().rexsc_int8_unpack(_ptr(self.data), self.rows, self.cols, _ptr(out), _stream(dev)),
+                       "rexsc_int8_unpack")
+        return out
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """``values() * scale`` in fp32, rounded to ``dtype``."""
+        return (self.values().float() * self.scale.unsqueeze(1)).to(dtype)
+
+
+def _int8_data(rows: int, cols: int, dev, what: str) -> torch.Tensor:
+    nbytes = _lib.load().rexsc_int8_data_size(rows, cols)
+    if nbytes == 0:
+        raise ValueError(f"{what}: unsupported size {rows} x {cols}")
+    return torch.empty(nbytes, dtype=torch.int8, device=dev)
+
+
+def _rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
+    """``t`` as [rows, cols] whose rows are dense (a view where that is possible)."""
+    t = _float_kind(t.detach())
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _int8_quantize(x: torch.Tensor, what: str) -> Int8Matrix:
+    rows, cols = x.shape
+    dev = x.device
+    data = _int8_data(rows, cols, dev, what)
+    scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    _lib.check(_lib.load().rexsc_int8_quantize(_ptr(x), _DTYPES[x.dtype], rows, cols, x.stride(0), _ptr(data), _ptr(scale),
+                                               _stream(dev)), "rexsc_int8_quantize")
+    return Int8Matrix(rows, cols, data, scale)
+
+
+@_traced
+def int8_quantize(x: torch.Tensor) -> Int8Matrix:
+    """Rows of ``x`` [rows, cols] (tokens of activations, output channels of weights) in 8-bit integers: the scale of a row is
+    ``max|x| / 127``, its integers are the exact quotients rounded to the nearest, ties to even.  A row of zeros has the scale
+    0; a row that holds an infinity or a NaN has the scale NaN and zeros, so that its products are NaN and no other row's."""
+    _require_cuda(x, "int8_quantize")
+    if x.dim() != 2 or 0 in x.shape or not x.is_floating_point():
+        raise ValueError("int8_quantize: expected floating-point [rows, cols], neither of them 0")
+    with _on(x.device):
+        return _int8_quantize(_rows_of(x, x.shape[1]), "int8_quantize")
+
+
+def _int8_bias(bias, n: int, dev, what: str):
+    """(tensor kept alive, pointer, dtype code)"""
+    if bias is None:
+        return None, 0, 0
+    if bias.device != dev or tuple(bias.shape) != (n,) or not bias.is_floating_point():
+        raise ValueError(f"{what}: expected a floating-point bias [{n}] on {dev}")
+    bias = _float_kind(bias.detach()).contiguous()
+    return bias, _ptr(bias), _DTYPES[bias.dtype]
+
+
+def _int8_matmul(a: Int8Matrix, b: Int8Matrix, bias, dtype: torch.dtype, what: str) -> torch.Tensor:
+    dev = a.device
+    keep, bias_ptr, bias_dtype = _int8_bias(bias, b.rows, dev, what)
+    out = torch.empty((a.rows, b.rows), dtype=dtype, device=dev)
+    _lib.check(_lib.load().rexsc_int8_matmul(_ptr(a.data), _ptr(a.scale), _ptr(b.data), _ptr(b.scale), bias_ptr, bias_dtype,
+                                             a.rows, b.rows, a.cols, _ptr(out), _DTYPES[dtype], _int8_kernel(), _stream(dev)),
+               "rexsc_int8_matmul")
+    del keep
+    return out
+
+
+@_traced
+def int8_matmul(a: Int8Matrix, b: Int8Matrix, bias: torch.Tensor = None, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """``a b^T`` [a.rows, b.rows]: exact sums of the products of the integers, times both rows' scales, plus ``bias``
+    [b.rows], in fp32 and rounded once to ``dtype`` (float32, float16 or bfloat16)."""
+    what = "int8_matmul"
+    if not isinstance(a, Int8Matrix) or not isinstance(b, Int8Matrix):
+        raise ValueError(f"{what}: expected two Int8Matrix operands")
+    if a.cols != b.cols or a.device != b.device:
+        raise ValueError(f"{what}: operands differ in columns ({a.cols}, {b.cols}) or device ({a.device}, {b.device})")
+    if dtype not in _DTYPES:
+        raise ValueError(f"{what}: dtype must be float32, float16 or bfloat16")
+    with _on(a.device):
+        return _int8_matmul(a, b, bias, dtype, what)
+
+
+class _Int8Linear(torch.autograd.Function):
+    """y = x w^T + bias with both operands in 8-bit integers; the gradients are products of 8-bit integers too."""
+
+    @staticmethod
+    def forward(ctx, x, weight, prepared, bias):
+        dev, n = x.device, (prepared or weight).shape[0]
+        x2 = _rows_of(x, x.shape[-1])
+        ctx.lead, ctx.dtypes = x.shape[:-1], (x.dtype, None if weight is None else weight.dtype,
+                                              None if bias is None else bias.dtype)
+        ctx.kernel = _int8_kernel()
+        if x2.shape[0] == 0:
+            ctx.sizes = (0, n, x.shape[-1])
+            return x2.new_empty((*ctx.lead, n))
+        with _on(dev):
+            w = prepared if prepared is not None else _int8_quantize(_rows_of(weight, weight.shape[1]), "int8_linear")
+            q = _int8_quantize(x2, "int8_linear")
+            y = _int8_matmul(q, w, bias, x2.dtype, "int8_linear")
+        ctx.sizes = (q.rows, n, q.cols)
+        ctx.save_for_backward(*((q.data, q.scale) if ctx.needs_input_grad[1] else (None, q.scale)),
+                              *((w.data, w.scale) if ctx.needs_input_grad[0] else (None, None)))
+        return y.view(*ctx.lead, n)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        m, n, k = ctx.sizes
+        want_dx, want_dw, _, want_db = ctx.needs_input_grad
+        xt, wt, bt = ctx.dtypes
+        dev = dy.device
+        with _on(dev):
+            kept = lambda t: t if t in _DTYPES else torch.float32
+            if m == 0:
+                zeros = lambda want, shape, t: torch.zeros(shape, dtype=t, device=dev) if want else None
+                return zeros(want_dx, (*ctx.lead, k), xt), zeros(want_dw, (n, k), wt), None, zeros(want_db, (n,), bt)
+            xd, xs, wd, ws = ctx.saved_tensors
+            lib = _lib.load()
+            g = _rows_of(dy, n)
+            dx = torch.empty((m, k), dtype=kept(xt), device=dev) if want_dx else None
+            dw = torch.empty((n, k), dtype=kept(wt), device=dev) if want_dw else None
+            db = torch.empty((n,), dtype=kept(bt), device=dev) if want_db else None
+            nbytes = lib.rexsc_int8_linear_bwd_workspace_size(m, n, want_dx, want_dw, want_db)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ptr = lambda t: 0 if t is None else _ptr(t)
+            code = lambda t: 0 if t is None else _DTYPES[t.dtype]
+            rc = lib.rexsc_int8_linear_bwd(_ptr(g), _DTYPES[g.dtype], m, n, k, g.stride(0), ptr(xd), ptr(xs), ptr(wd), ptr(ws),
+                                           ptr(dx), code(dx), ptr(dw), code(dw), ptr(db), code(db), ctx.kernel,
+                                           _ptr(scratch), nbytes, _stream(dev))
+            _lib.check(rc, "rexsc_int8_linear_bwd")
+            return (None if dx is None else dx.view(*ctx.lead, k).to(xt), None if dw is None else dw.to(wt), None,
+                    None if db is None else db.to(bt))
+
+
+@_traced
+def int8_linear(x: torch.Tensor, weight, bias: torch.Tensor = None) -> torch.Tensor:
+    """A linear layer in 8-bit integers: ``x`` [..., k] is quantised per token, multiplied with ``weight`` and returned in
+    ``x``'s type as [..., n].  The plain digital form of the layer that :func:`linear_generic_general_acc` computes on
+    bit streams.
+
+    ``weight``: an :class:`Int8Matrix` [n, k], quantised once per output channel (serving); or a floating-point tensor [n, k]
+    that is quantised in the call (training).  Gradients flow to ``x``, to a floating-point ``weight`` and to ``bias``, past
+    the rounding of either operand as if it were not there.  They are products of 8-bit integers as well:
+    with ``dx = dy w`` and ``dw = dy^T x`` the scales of the operand that the sum runs over are folded into ``dy`` (in fp32),
+    which is then quantised per token for ``dx`` and per output channel for ``dw``; the bias's gradient is the plain sum.
+
+    Sums are exact up to 131071 products: ``k``, and in training ``n`` (for ``dx``) and the number of tokens (for ``dw``).
+
+    Both directions can be captured into a CUDA graph; every call has scratch of its own.  As with any op of torch, drop all
+    eager graphs of the same leaves (outputs that still hold one) before capturing a backward pass: torch's engine would wait
+    on the stream of their leaf nodes, which ends the capture, or the process, with an error."""
+    what = "int8_linear"
+    _require_cuda(x, what)
+    prepared = isinstance(weight, Int8Matrix)
+    if not prepared:
+        _require_cuda(weight, what)
+        if weight.dim() != 2 or not weight.is_floating_point():
+            raise ValueError(f"{what}: expected a floating-point weight [n, k] or an Int8Matrix")
+    n, k = weight.shape
+    if x.dim() < 1 or x.shape[-1] != k or n == 0 or k == 0 or not x.is_floating_point():
+        raise ValueError(f"{what}: expected floating-point x [..., {k}] for weights [{n}, {k}], neither of them 0")
+    if weight.device != x.device:
+        raise ValueError(f"{what}: x is on {x.device}, the weights are on {weight.device}")
+    if k > _lib.INT8_MAX_DOT:
+        raise ValueError(f"{what}: sums of more than {_lib.INT8_MAX_DOT} products are not supported (k = {k})")
+    if torch.is_grad_enabled() and (x.requires_grad or (not prepared and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        _int8_bias(bias, n, x.device, what)
+        if x.requires_grad and n > _lib.INT8_MAX_DOT:
+            raise ValueError(f"{what}: the gradient of x sums over {n} output channels, at most {_lib.INT8_MAX_DOT}")
+        if not prepared and weight.requires_grad and x.numel() // k > _lib.INT8_MAX_DOT:
+            raise ValueError(f"{what}: the weight's gradient sums over {x.numel() // k} tokens, at most {_lib.INT8_MAX_DOT}")
+        return _Int8Linear.apply(x, None if prepared else weight, weight if prepared else None, bias)
+    dev = x.device
+    lib = _lib.load()
+    with _on(dev):
+        x2 = _rows_of(x, k)
+        m = x2.shape[0]
+        keep, bias_ptr, bias_dtype = _int8_bias(bias, n, dev, what)
+        out = torch.empty((m, n), dtype=x2.dtype, device=dev)
+        if m:
+            w = weight if prepared else _int8_quantize(_rows_of(weight, k), what)
+            nbytes = lib.rexsc_int8_linear_workspace_size(m, k)
+            if nbytes == 0:
+                raise ValueError(f"{what}: unsupported size {m} x {k}")
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            rc = lib.rexsc_int8_linear_fwd(_ptr(x2), _DTYPES[x2.dtype], m, k, x2.stride(0), _ptr(w.data), _ptr(w.scale), n,
+                                           bias_ptr, bias_dtype, _ptr(out), _DTYPES[x2.dtype], _int8_kernel(),
+                                           _ptr(scratch), nbytes, _stream(dev))
+            _lib.check(rc, "rexsc_int8_linear_fwd")
+            if _DEBUG:
+                _lib.check(lib.rexsc_int8_status(_stream(dev)), "rexsc_int8_linear_fwd (device status)")
+    del keep
+    return out.view(*x.shape[:-1], n)
+
+
+def int8_status(device=None) -> int:
+    """Synchronise the current stream and return 0, or -6 if a bounded device-side wait of an int8 product gave up since the
+    last call (its outputs are then incomplete)."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with _on(dev):
+        return _lib.load().rexsc_int8_status(_stream(dev))
+
+
 # ---- helpers used by tests and the benchmark ------------------------------------------------------------
 def build_lfsr_lut(lfsr_length: int, bit_length: int, gen_config: int = 1, xnor: bool = True,
                    prog_load: Sequence[int] = (7, 8, 1), is_weight: bool = False, device="cuda") -> torch.Tensor:
