@@ -1,8 +1,8 @@
 // Products of 8-bit matrices with scales per row and per column, on the 5th-generation tensor cores:
 //   out[i, j] = (sum_k a[i, k] b[j, k]) * row_scale[i] * col_scale[j] + bias[j],
 // the sum exact in int32 (tcgen05.mma.kind::i8, accumulators in TMEM), the rest in fp32, rounded once to the output's type.
-// Operands are tiled and swizzled in memory (int8.cuh), so a pipeline stage is one or two contiguous bulk copies of at most
-// 16 KiB, needs no tensor map, and a matrix serves K-major or MN-major by a bit of the instruction descriptor.
+// Operands are tiled and swizzled in memory (int8.cuh), so a pipeline stage is two contiguous copies of at most 16 KiB each,
+// and a matrix serves K-major or MN-major by a bit of the instruction descriptor.
 //
 // Two kernels:
 //   product_pair_kernel  pairs of CTAs (cta_group::2) on 256 x 256 output tiles, persistent, two accumulators per CTA so that
@@ -12,6 +12,8 @@
 //                        order does not matter).
 // Every mbarrier wait is bounded; a CTA whose wait gives up raises the library's status word (rexsc_int8_status), stores
 // nothing more, waits for its copies in flight, frees its TMEM and leaves.
+#include <cuda.h>
+
 #include "int8.cuh"
 
 namespace rexsc {
@@ -28,14 +30,13 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
 {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-// (acquire at cluster scope: some arrivals come from the other CTA of a pair)
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity)
 {
     for (uint32_t i = 0; i < kWaitLimit; i++) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
@@ -53,14 +54,24 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank)
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(addr), "r"(rank));
     return out;
 }
+// (orders nothing but TMEM reads, which tcgen05.wait::ld and the fence before it have finished)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mapped)
 {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapped) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapped) : "memory");
 }
 __device__ __forceinline__ void copy_in(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
 {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                  "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// A tile of a matrix of tiles (rows of 128 bytes) into this CTA's shared memory, its bytes counted by a barrier of either CTA of
+// the pair: the leader's barrier then covers both CTAs' stages.  (Passing the word on by a remote arrive at cluster scope
+// instead cost 900 to 1500 cycles a stage: 8192^3 in 946 us.)
+__device__ __forceinline__ void copy_tile_pair(uint32_t dst, const CUtensorMap *map, int row, uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(0), "r"(row) : "memory");
 }
 __device__ __forceinline__ void cluster_sync()
 {
@@ -143,6 +154,7 @@ __device__ __forceinline__ float scaled(int sum, float row, float col, float bia
 }
 
 struct PairArgs {
+    CUtensorMap map_a, map_b;   // the operands as rows of 128 bytes
     I8Product p;
     long long tiles_i, tiles_j; // 256 x 256 output tiles
     int k_blocks;
@@ -226,7 +238,7 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; s++) {
-            mbar_init(full(s), rank == 0 ? 2 : 1); // the leader's: its own copies and the word that the other's have landed
+            mbar_init(full(s), 1); // (the leader's counts both CTAs' bytes, the other's is not used)
             mbar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; b++) mbar_init(acc_full(b), 1), mbar_init(acc_empty(b), 8); // four warps of each CTA
@@ -244,9 +256,20 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
     const uint32_t tmem = *tmem_slot;
     wait_previous_launch();
 
+    // stage and its phase, advanced together: a division in these loops costs as much as a copy
+    struct Ring {
+        uint32_t at = 0, phase = 0;
+        __device__ __forceinline__ void next()
+        {
+            if (++at == kPairStages) at = 0, phase ^= 1;
+        }
+    };
     if (warp == 0) {
         if (lane == 0) { // ---- copies
-            uint32_t it = 0;
+            const int step_a = (int)a.p.a.step_k * kI8Tile, step_b = (int)a.p.b.step_k * kI8Tile;
+            const uint32_t smem0 = smem_addr(smem), leader_full = map_rank(full(0), 0);
+            Ring r;
+            uint32_t filled = 0; // stages that have been used
             bool ok = true;
             for (long long t = first; t < tiles && ok; t += step) {
                 long long ti, tj;
@@ -255,46 +278,43 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
                 long long ia = ti * 2 + rank, ib = tj * 2 + rank;
                 ia = ia < a.p.a.mn_tiles ? ia : a.p.a.mn_tiles - 1;
                 ib = ib < a.p.b.mn_tiles ? ib : a.p.b.mn_tiles - 1;
-                const int8_t *pa = a.p.a.data + (size_t)(ia * a.p.a.step_mn) * kI8TileBytes;
-                const int8_t *pb = a.p.b.data + (size_t)(ib * a.p.b.step_mn) * kI8TileBytes;
-                for (int k = 0; k < a.k_blocks; k++, it++) {
-                    const int s = it % kPairStages;
-                    if (it >= kPairStages && !(ok = mbar_wait(empty(s), (it / kPairStages - 1) & 1))) break;
-                    const uint32_t dst = smem_addr(smem) + s * kPairStageBytes;
-                    mbar_expect(full(s), kPairStageBytes);
-                    copy_in(dst, pa + (size_t)(k * a.p.a.step_k) * kI8TileBytes, kI8TileBytes, full(s));
-                    copy_in(dst + kI8TileBytes, pb + (size_t)(k * a.p.b.step_k) * kI8TileBytes, kI8TileBytes, full(s));
+                int row_a = (int)(ia * a.p.a.step_mn) * kI8Tile, row_b = (int)(ib * a.p.b.step_mn) * kI8Tile;
+                for (int k = a.k_blocks; k > 0; k--) {
+                    if (filled == kPairStages) {
+                        if (!(ok = mbar_wait(empty(r.at), r.phase ^ 1))) break;
+                    } else {
+                        filled++;
+                    }
+                    const uint32_t dst = smem0 + r.at * kPairStageBytes, bar = leader_full + r.at * 8;
+                    if (rank == 0) mbar_expect(full(r.at), 2 * kPairStageBytes);
+                    copy_tile_pair(dst, &a.map_a, row_a, bar);
+                    copy_tile_pair(dst + kI8TileBytes, &a.map_b, row_b, bar);
+                    row_a += step_a, row_b += step_b;
+                    r.next();
                 }
             }
-            // nothing on its way when this CTA leaves (at once, unless a wait gave up somewhere)
-            for (uint32_t j = it < kPairStages ? 0 : it - kPairStages; j < it; j++) mbar_wait(full(j % kPairStages), (j / kPairStages) & 1);
+            // nothing on its way to either CTA when they leave (at once, unless a wait gave up somewhere)
+            for (uint32_t j = 0; rank == 0 && j < filled; j++) {
+                const bool before = filled == kPairStages && j >= r.at; // last filled in the turn before this one
+                mbar_wait(full(j), before ? r.phase ^ 1 : r.phase);
+            }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 1) { // ---- tell the leader that this CTA's copies have landed
-            uint32_t it = 0;
-            bool ok = true;
-            for (long long t = first; t < tiles && ok; t += step)
-                for (int k = 0; k < a.k_blocks; k++, it++) {
-                    const int s = it % kPairStages;
-                    if (!(ok = mbar_wait(full(s), (it / kPairStages) & 1))) break;
-                    mbar_arrive_cluster(map_rank(full(s), 0));
-                }
-        } else if (lane == 0) { // ---- products
+        if (lane == 0 && rank == 0) { // ---- products
             const uint32_t idesc = product_idesc(256, 256, a.p.a.mn_major, a.p.b.mn_major);
             const uint32_t adv_a = a.p.a.mn_major ? 4096 >> 4 : 32 >> 4, adv_b = a.p.b.mn_major ? 4096 >> 4 : 32 >> 4;
-            uint32_t it = 0;
+            const uint64_t desc0 = tile_desc(smem_addr(smem));
+            Ring r;
             int turn = 0;
             bool ok = true;
             for (long long t = first; t < tiles && ok; t += step, turn++) {
                 const int b = turn & 1;
                 if (turn >= 2 && !(ok = mbar_wait(acc_empty(b), (turn / 2 - 1) & 1))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int k = 0; k < a.k_blocks; k++, it++) {
-                    const int s = it % kPairStages;
-                    if (!(ok = mbar_wait(full(s), (it / kPairStages) & 1))) break;
+                for (int k = 0; k < a.k_blocks; k++) {
+                    if (!(ok = mbar_wait(full(r.at), r.phase))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t sa = smem_addr(smem) + s * kPairStageBytes;
-                    const uint64_t da = tile_desc(sa), db = tile_desc(sa + kI8TileBytes);
+                    const uint64_t da = desc0 + r.at * (kPairStageBytes >> 4), db = da + (kI8TileBytes >> 4);
 #pragma unroll
                     for (int q = 0; q < 4; q++)
                         asm volatile(
@@ -303,7 +323,8 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
                             "l"(da + q * adv_a), "l"(db + q * adv_b), "r"(idesc), "r"((uint32_t)(k | q)) : "memory");
                     asm volatile(
                         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                            empty(s)), "h"((uint16_t)3) : "memory");
+                            empty(r.at)), "h"((uint16_t)3) : "memory");
+                    r.next();
                 }
                 if (ok)
                     asm volatile(
@@ -333,7 +354,9 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
             }
             const float rs = row < a.p.m ? a.p.row_scale[row] : 0.f;
             asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (!mbar_wait(acc_full(b), (turn / 2) & 1)) break;
+            // one lane of a warp asks: 128 threads that poll cost the copying thread a fifth of its rate
+            const bool there = lane != 0 || mbar_wait(acc_full(b), (turn / 2) & 1);
+            if (!__all_sync(0xffffffffu, there)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
             for (int c = 0; c < 256; c += 32) {
@@ -599,11 +622,38 @@ int launch_cluster(void (*kernel)(Args), const Args &args, long long blocks, int
     return REXSC_OK;
 }
 
+// a matrix of tiles as rows of 128 bytes, taken 128 rows at a time
+int tile_map(CUtensorMap *map, const I8Operand &o, long long k_tiles)
+{
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<Encode>(fn);
+    }();
+    const long long rows = o.mn_tiles * k_tiles * kI8Tile;
+    if (!encode || rows > 0x7fffffffll) return REXSC_E_UNSUPPORTED;
+    const cuuint64_t extent[2] = {kI8Tile, (cuuint64_t)rows}, pitch[1] = {kI8Tile};
+    const cuuint32_t box[2] = {kI8Tile, kI8Tile}, each[2] = {1, 1};
+    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(o.data), extent, pitch, box, each,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return rc == CUDA_SUCCESS ? REXSC_OK : REXSC_E_BAD_ARG;
+}
+
 template <typename T>
 int launch_pair(const I8Product &p, bool overlap, cudaStream_t st)
 {
     PairArgs a;
     a.p = p;
+    int rc = tile_map(&a.map_a, p.a, i8_tiles(p.k));
+    if (rc == REXSC_OK) rc = tile_map(&a.map_b, p.b, i8_tiles(p.k));
+    if (rc != REXSC_OK) return rc;
     a.tiles_i = (p.m + 255) / 256;
     a.tiles_j = (p.n + 255) / 256;
     a.k_blocks = (int)i8_tiles(p.k);
