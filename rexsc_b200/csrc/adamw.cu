@@ -19,7 +19,9 @@
 // 2^-100 is stored as zeros.  A gradient that is no finite number makes its element's moments so, and in 8 bits its block's.
 //
 // What bounds it: memory.  Per element 28 bytes (fp32 weights and gradients, 32-bit moments), 16 with 8-bit moments.
+#include <cuda_fp8.h>
 #include <math.h>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -28,7 +30,9 @@ namespace rexsc {
 namespace {
 
 constexpr int kBlock = 256;      // elements of a block (of a scale)
-constexpr int kThreads = 256;
+// With 8-bit moments the arithmetic needs 96 registers a thread: five CTAs of 128 threads fit an SM (two of 256: 4 % slower).
+template <bool kBits8> constexpr int kThreadsOf = kBits8 ? 128 : 256;
+template <bool kBits8> constexpr int kCtasOf = kBits8 ? 5 : 3;
 constexpr int kSmallList = 64, kLargeList = 640;
 
 struct AdamTensor {
@@ -62,23 +66,52 @@ __device__ __forceinline__ void load8v(const float *p, float (&v)[8])
     asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(p));
 }
-__device__ __forceinline__ void load8v(const __half *p, float (&v)[8])
+// Eight neighbouring elements as they lie in memory (16-bit types: in the first four words)
+struct Raw8 {
+    uint32_t w[8];
+};
+__device__ __forceinline__ void load_raw(const void *p, int dtype, Raw8 &r)
 {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    if (dtype == REXSC_F32) {
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+                     : "l"(p));
+    } else {
+        const uint4 u = *static_cast<const uint4 *>(p);
+        r.w[0] = u.x, r.w[1] = u.y, r.w[2] = u.z, r.w[3] = u.w;
     }
 }
-__device__ __forceinline__ void load8v(const __nv_bfloat16 *p, float (&v)[8])
+// one at a time, `left` of them; the others are 0
+__device__ __forceinline__ void load_some(const void *p, int dtype, int left, Raw8 &r)
 {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if (dtype == REXSC_F32) {
+        const uint32_t *q = static_cast<const uint32_t *>(p);
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        for (int i = 0; i < 8; i++) r.w[i] = i < left ? q[i] : 0u;
+    } else {
+        const uint16_t *q = static_cast<const uint16_t *>(p);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            r.w[i] = (2 * i < left ? (uint32_t)q[2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)q[2 * i + 1] << 16 : 0u);
+    }
 }
+__device__ __forceinline__ void widen(const Raw8 &r, int dtype, float (&v)[8])
+{
+    if (dtype == REXSC_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r.w[i]);
+    } else if (dtype == REXSC_F16) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r.w[i]));
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[2 * i] = __uint_as_float(r.w[i] << 16), v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+    }
+}
+template <typename T> constexpr int kDtypeOf = sizeof(T) == 4 ? REXSC_F32 : std::is_same<T, __half>::value ? REXSC_F16 : REXSC_BF16;
 __device__ __forceinline__ void store8v(float *p, const float (&v)[8])
 {
     asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
@@ -103,36 +136,68 @@ template <> __device__ __forceinline__ float narrow<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// elements [e, e + 8) of a tensor of n; zeros behind its end
-template <typename T>
-__device__ __forceinline__ void load_elems(const T *p, long long e, long long n, int vec, float (&v)[8])
+// eight e4m3 codes (4 exponent bits with bias 7, 3 of mantissa, steps of 2^-9 below 2^-6), times a scale
+__device__ __forceinline__ void from_e4m3(uint2 codes, float scale, float (&v)[8])
 {
-    if (vec && e + 8 <= n) {
-        load8v(p + e, v);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = e + i < n ? load_as_float(p + e + i, 0) : 0.f;
+    for (int i = 0; i < 4; i++) {
+        const uint32_t pair = i < 2 ? codes.x : codes.y;
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(i & 1 ? pair >> 16 : pair & 0xffff), __NV_E4M3);
+        const float2 f = __half22float2(__half2(h));
+        v[2 * i] = __fmul_rn(f.x, scale), v[2 * i + 1] = __fmul_rn(f.y, scale);
     }
 }
-
-// e4m3 <-> fp32 by the bits: 4 exponent bits (bias 7), 3 of mantissa, steps of 2^-9 below 2^-6
-__device__ __forceinline__ float from_e4m3(uint32_t code) // (sign in bit 7; the two NaN codes come out as NaN)
+// y in [0, 448] to e4m3, rounded up by the threshold u / 2^20.  From 2^-6 on the fraction is the low 20 bits of y's mantissa;
+// below, steps are 2^-9 and the fraction that of y * 2^9 plus the threshold, a sum in fp32 whose whole part an addition of
+// 2^23 that rounds down leaves in the low bits.  (Only the low byte counts; its sign bit is 0.)
+__device__ __forceinline__ uint32_t to_e4m3_normal(float y, uint32_t u) { return (__float_as_uint(y) + u - ((127u - 7u) << 23)) >> 20; }
+__device__ __forceinline__ uint32_t to_e4m3_small(float y, uint32_t u)
 {
-    const uint32_t mag = code & 0x7f;
-    const float v = mag >= 8 ? __uint_as_float((mag << 20) + ((127 - 7) << 23)) : (float)mag * 0x1p-9f;
-    const float w = mag == 0x7f ? __uint_as_float(0x7fc00000u) : v;
-    return code & 0x80 ? -w : w;
+    const float part = __fadd_rn(__uint_as_float(0x3f800000u | u << 3), -1.f);
+    return __float_as_uint(__fadd_rd(__fmaf_rn(y, 512.f, part), 8388608.f));
 }
-// y in [0, 448 (1 + 2^-22)], u < 2^20
-__device__ __forceinline__ uint32_t to_e4m3(float y, uint32_t u)
+// byte `at` of four words
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t at)
 {
-    const uint32_t normal = ((__float_as_uint(y) + u) >> 20) - ((127 - 7) << 3);
-    const uint32_t small = (uint32_t)__float2int_rd(__fadd_rn(__fmul_rn(y, 512.f), __fmul_rn((float)u, 0x1p-20f)));
-    return min(y < 0x1p-6f ? small : normal, 126u);
+    const uint32_t sel = at | (at + 4) << 4;
+    return __byte_perm(__byte_perm(a, b, sel), __byte_perm(c, d, sel), 0x5410);
+}
+// Eight magnitudes x, in units whose reciprocal is `per`, as e4m3; least: what is not 0 is not stored as 0.  Blocks whose
+// values all lie above 2^-6 (1 / 28672 of the largest) skip the small steps: 96 -> 50 instructions an element.
+__device__ __forceinline__ uint2 store_e4m3(const float (&x)[8], float most, float per, const uint32_t (&u)[8], bool least)
+{
+    float y[8], low = 448.f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        y[i] = __fmul_rn(fabsf(x[i]), per);
+        low = fminf(low, y[i]);
+    }
+    if (!(__fmul_rn(most, per) <= 448.f)) { // (the same for the block) rounding has put the largest above the largest code
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = fminf(y[i], 448.f);
+    }
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) c[i] = to_e4m3_normal(y[i], u[i]);
+    if (low < 0x1p-6f) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (y[i] < 0x1p-6f) c[i] = to_e4m3_small(y[i], u[i]) & 0xff;
+            if (least && y[i] > 0.f) c[i] = max(c[i], 1u);
+        }
+    }
+    return make_uint2(pack4(c[0], c[1], c[2], c[3], 0), pack4(c[4], c[5], c[6], c[7], 0));
+}
+__device__ __forceinline__ float reciprocal(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-template <typename P, bool kBits8, int kList>
-__global__ void __launch_bounds__(kThreads)
+// kSame: gradients have the weights' type (known here: a tenth of the time with 8-bit moments)
+template <typename P, bool kBits8, bool kSame, int kList>
+__global__ void __launch_bounds__(kThreadsOf<kBits8>, kCtasOf<kBits8>)
 adamw_kernel(const __grid_constant__ AdamLaunch<kList> l)
 {
     const AdamArgs &a = l.a;
@@ -144,37 +209,78 @@ adamw_kernel(const __grid_constant__ AdamLaunch<kList> l)
     const float keep = 1.f - lr * a.wd;
     const float size = lr / -expm1f((float)((double)t * a.log_b1));
     const float root = rsqrtf(-expm1f((float)((double)t * a.log_b2)));
-    const unsigned warps = gridDim.x * (kThreads / 32);
-    int at = 0;
-    for (unsigned b = a.first + blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); b < a.last; b += warps) {
-        // the last tensor that begins at b or before; blocks only rise, so the search goes on from where it was
-        if (at + 1 < a.tensors && l.t[at + 1].first <= b) {
-            int lo = at + 1, hi = a.tensors;
+    constexpr int kWarps = kThreadsOf<kBits8> / 32;
+    const unsigned warps = gridDim.x * kWarps;
+
+    // A block's inputs.  With 8-bit moments those of the next one are under way during the computation for this one, which
+    // is long enough that the warps an SM holds would not cover the memory's latency.
+    struct Block {
+        P *p_at;  // this lane's elements of the weights
+        int left; // how many of its eight exist; -1: a block of no tensor of the list
+        int vec;
+        Raw8 p, g;
+        uint2 cm, cr;
+        float sm, sr;
+    };
+    // the tensor that blocks are taken from: its blocks, and its pointers as if it began at block 0 (the flat buffers' place
+    // is then its offset too; most blocks need nothing else)
+    int at = -1;
+    unsigned first = 0, end = 0, whole = 0; // whole: blocks up to here lie wholly in the tensor
+    P *p_base = nullptr;
+    const char *g_base = nullptr;
+    const int g_dtype = kSame ? kDtypeOf<P> : a.g_dtype, g_size = g_dtype == REXSC_F32 ? 4 : 2;
+    auto load = [&](unsigned b, Block &x) {
+        if (b >= end) {
+            // the last tensor that begins at b or before; blocks only rise, so the search goes on from where it was
+            int lo = at < 0 ? 0 : at, hi = a.tensors;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (l.t[mid].first <= b) lo = mid; else hi = mid;
             }
-            at = lo;
-        }
-        const AdamTensor &x = l.t[at];
-        if ((long long)(b - x.first) * kBlock >= x.n) continue; // a block of no tensor of the list
-        const long long e = (long long)(b - x.first) * kBlock + lane * 8; // in the tensor
-        const size_t pos = (size_t)b * kBlock + lane * 8;                 // in the flat buffers
-        P *px = static_cast<P *>(x.p);
-        float p[8], g[8], m[8], v[8];
-        load_elems(px, e, x.n, x.vec, p);
-        if (a.g_dtype == REXSC_F32) load_elems(static_cast<const float *>(x.g), e, x.n, x.vec, g);
-        else if (a.g_dtype == REXSC_F16) load_elems(static_cast<const __half *>(x.g), e, x.n, x.vec, g);
-        else load_elems(static_cast<const __nv_bfloat16 *>(x.g), e, x.n, x.vec, g);
-        if constexpr (kBits8) {
-            const uint2 cm = *reinterpret_cast<const uint2 *>(a.m8 + pos), cr = *reinterpret_cast<const uint2 *>(a.r8 + pos);
-            const float sm = a.ms[b], sr = a.rs[b];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                m[i] = __fmul_rn(from_e4m3((i < 4 ? cm.x : cm.y) >> (8 * (i & 3)) & 0xff), sm);
-                const float r = __fmul_rn(from_e4m3((i < 4 ? cr.x : cr.y) >> (8 * (i & 3)) & 0xff), sr);
-                v[i] = __fmul_rn(r, r);
+            if (lo != at) {
+                at = lo;
+                const AdamTensor &t = l.t[lo];
+                first = t.first;
+                end = first + (unsigned)((t.n + kBlock - 1) / kBlock);
+                whole = t.vec ? first + (unsigned)(t.n / kBlock) : first;
+                p_base = static_cast<P *>(t.p) - (size_t)first * kBlock;
+                g_base = static_cast<const char *>(t.g) - (size_t)first * kBlock * g_size;
             }
+            if (b >= end) {
+                x.left = -1;
+                return;
+            }
+        }
+        const size_t pos = (size_t)b * kBlock + lane * 8;
+        x.p_at = p_base + pos;
+        const char *g_at = g_base + pos * g_size;
+        if (b < whole) {
+            x.left = 8, x.vec = 1;
+            load_raw(x.p_at, kDtypeOf<P>, x.p);
+            load_raw(g_at, g_dtype, x.g);
+        } else {
+            const AdamTensor &t = l.t[at];
+            const long long left = t.n - ((long long)(b - first) * kBlock + lane * 8);
+            x.left = left < 0 ? 0 : left < 8 ? (int)left : 8, x.vec = t.vec;
+            load_some(x.p_at, kDtypeOf<P>, x.left, x.p);
+            load_some(g_at, g_dtype, x.left, x.g);
+        }
+        if constexpr (kBits8) {
+            x.cm = *reinterpret_cast<const uint2 *>(a.m8 + pos), x.cr = *reinterpret_cast<const uint2 *>(a.r8 + pos);
+            x.sm = a.ms[b], x.sr = a.rs[b];
+        }
+    };
+    auto update = [&](unsigned b, const Block &x) {
+        if (x.left < 0) return;
+        const size_t pos = (size_t)b * kBlock + lane * 8; // in the flat buffers
+        float p[8], g[8], m[8], v[8];
+        widen(x.p, kDtypeOf<P>, p);
+        widen(x.g, g_dtype, g);
+        if constexpr (kBits8) {
+            from_e4m3(x.cm, x.sm, m);
+            from_e4m3(x.cr, x.sr, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = __fmul_rn(v[i], v[i]);
         } else {
             load8v(a.m + pos, m);
             load8v(a.v + pos, v);
@@ -187,42 +293,54 @@ adamw_kernel(const __grid_constant__ AdamLaunch<kList> l)
             m[i] = __fadd_rn(__fmul_rn(a.b1, m[i]), __fmul_rn(a.c1, g[i]));
             v[i] = __fadd_rn(__fmul_rn(a.b2, v[i]), __fmul_rn(a.c2, __fmul_rn(g[i], g[i])));
             r[i] = __fsqrt_rn(v[i]);
-            p[i] = p[i] * keep - __fdividef(size * m[i], fmaf(r[i], root, a.eps));
+            // (the divisor is 0, or neither below 2^-74 nor above 2^84 / sqrt(1 - b2))
+            p[i] = fmaf(-size * m[i], reciprocal(fmaf(r[i], root, a.eps)), p[i] * keep);
         }
-        if (x.vec && e + 8 <= x.n) {
-            store8v(px + e, p);
+        if (x.vec && x.left == 8) {
+            store8v(x.p_at, p);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (e + i < x.n) px[e + i] = narrow<P>(p[i]);
+                if (i < x.left) x.p_at[i] = narrow<P>(p[i]);
         }
         if constexpr (kBits8) {
             uint32_t am = 0, ar = 0; // bits: a NaN is larger than everything
 #pragma unroll
-            for (int i = 0; i < 8; i++) am = max(am, __float_as_uint(m[i]) & 0x7fffffffu), ar = max(ar, __float_as_uint(r[i]) & 0x7fffffffu);
+            for (int i = 0; i < 8; i++) am = max(am, __float_as_uint(m[i]) & 0x7fffffffu), ar = max(ar, __float_as_uint(r[i]));
             const float most_m = __uint_as_float(__reduce_max_sync(0xffffffffu, am)), most_r = __uint_as_float(__reduce_max_sync(0xffffffffu, ar));
-            const float per_m = most_m < 0x1p-100f ? 0.f : __fdiv_rn(448.f, most_m), per_r = most_r < 0x1p-100f ? 0.f : __fdiv_rn(448.f, most_r);
-            if (lane == 0) {
-                a.ms[b] = most_m < 0x1p-100f ? 0.f : __fdiv_rn(most_m, 448.f);
-                a.rs[b] = most_r < 0x1p-100f ? 0.f : __fdiv_rn(most_r, 448.f);
-            }
-            uint32_t wm[2] = {0, 0}, wr[2] = {0, 0};
+            // the block's four quotients, one to a lane
+            const float most = lane & 1 ? most_r : most_m;
+            float quotient = __fdiv_rn(lane & 2 ? most : 448.f, lane & 2 ? 448.f : most);
+            if (most < 0x1p-100f) quotient = 0.f;
+            const float per_m = __shfl_sync(0xffffffffu, quotient, 0), per_r = __shfl_sync(0xffffffffu, quotient, 1);
+            if (lane == 2) a.ms[b] = quotient;
+            if (lane == 3) a.rs[b] = quotient;
             const uint32_t u0 = (uint32_t)pos * 0xC13FA9A9u + (uint32_t)t * 0x9E3779B9u;
+            uint32_t u[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint32_t u = u0 + i * 0xC13FA9A9u;
-                const uint32_t code_m = to_e4m3(__fmul_rn(fabsf(m[i]), per_m), u >> 12) | (__float_as_uint(m[i]) >> 31) << 7;
-                const float y = __fmul_rn(r[i], per_r);
-                const uint32_t code_r = max(to_e4m3(y, ~u >> 12), y > 0.f ? 1u : 0u);
-                wm[i >> 2] |= code_m << (8 * (i & 3));
-                wr[i >> 2] |= code_r << (8 * (i & 3));
-            }
-            *reinterpret_cast<uint2 *>(a.m8 + pos) = make_uint2(wm[0], wm[1]);
-            *reinterpret_cast<uint2 *>(a.r8 + pos) = make_uint2(wr[0], wr[1]);
+            for (int i = 0; i < 8; i++) u[i] = (u0 + i * 0xC13FA9A9u) >> 12;
+            uint2 wm = store_e4m3(m, most_m, per_m, u, false);
+            auto sign = [&](int i) { return __float_as_uint(m[i]); };
+            wm.x |= pack4(sign(0), sign(1), sign(2), sign(3), 3) & 0x80808080u;
+            wm.y |= pack4(sign(4), sign(5), sign(6), sign(7), 3) & 0x80808080u;
+#pragma unroll
+            for (int i = 0; i < 8; i++) u[i] = 0xfffffu - u[i];
+            *reinterpret_cast<uint2 *>(a.m8 + pos) = wm;
+            *reinterpret_cast<uint2 *>(a.r8 + pos) = store_e4m3(r, most_r, per_r, u, true);
         } else {
             store8v(a.m + pos, m);
             store8v(a.v + pos, v);
         }
+    };
+    unsigned b = a.first + blockIdx.x * kWarps + (threadIdx.x >> 5);
+    Block now, next;
+    if (kBits8 && b < a.last) load(b, now);
+    for (; b < a.last; b += warps) {
+        if (!kBits8) load(b, now);
+        else if (b + warps < a.last) load(b + warps, next);
+        const Block x = now;
+        now = next;
+        update(b, x);
     }
     // the last block of the launch to get here counts the step: all others have read the count
     if (a.advance) {
@@ -248,18 +366,22 @@ int launch_list(const AdamArgs &a, const rexsc_adamw_tensor *list, cudaStream_t 
                               !(reinterpret_cast<uintptr_t>(list[i].d_param) & p_align) &&
                                   !(reinterpret_cast<uintptr_t>(list[i].d_grad) & g_align)};
     };
-    const long long blocks = ((long long)a.last - a.first + kThreads / 32 - 1) / (kThreads / 32);
-    const unsigned grid = (unsigned)(blocks < 148 * 8 ? blocks : 148 * 8);
+    constexpr int kThreads = kThreadsOf<kBits8>, kWarps = kThreads / 32;
+    const long long blocks = ((long long)a.last - a.first + kWarps - 1) / kWarps;
+    const unsigned most = 148 * (kBits8 ? kCtasOf<true> : 8), grid = (unsigned)(blocks < most ? blocks : most);
+    const bool same = a.g_dtype == kDtypeOf<P>;
     if (a.tensors <= kSmallList) {
         AdamLaunch<kSmallList> l;
         l.a = a;
         fill(l.t);
-        adamw_kernel<P, kBits8, kSmallList><<<grid, kThreads, 0, st>>>(l);
+        if (same) adamw_kernel<P, kBits8, true, kSmallList><<<grid, kThreads, 0, st>>>(l);
+        else adamw_kernel<P, kBits8, false, kSmallList><<<grid, kThreads, 0, st>>>(l);
     } else {
         AdamLaunch<kLargeList> l;
         l.a = a;
         fill(l.t);
-        adamw_kernel<P, kBits8, kLargeList><<<grid, kThreads, 0, st>>>(l);
+        if (same) adamw_kernel<P, kBits8, true, kLargeList><<<grid, kThreads, 0, st>>>(l);
+        else adamw_kernel<P, kBits8, false, kLargeList><<<grid, kThreads, 0, st>>>(l);
     }
     REXSC_LAUNCH_CHECK("adamw_kernel");
     return REXSC_OK;

@@ -7,14 +7,24 @@ place in ``utils_own.train``: it is a ``torch.optim.Optimizer``, so learning-rat
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import Dict
 
 import numpy as np
 import torch
 
+try:
+    from torch.optim.optimizer import _global_optimizer_post_hooks as _POST_HOOKS
+    from torch.optim.optimizer import _global_optimizer_pre_hooks as _PRE_HOOKS
+except ImportError:  # a torch without hooks for all optimizers
+    _PRE_HOOKS, _POST_HOOKS = {}, {}
+
 from . import _lib
 from .ops import _DTYPES, _on, _stream
 
+_STRIDED = torch.strided
+_stride, _numel, _data_ptr, _dtype = (torch.Tensor.stride, torch.Tensor.numel, torch.Tensor.data_ptr,
+                                      operator.attrgetter("dtype"))
 BLOCK = 256  # elements of a block of the flat moment buffers (of a scale of 8-bit moments)
 
 
@@ -96,7 +106,14 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     views[name] = t[a:b].as_strided(p.shape, p.stride()) if b > a else t[a:b].view(p.shape)
             self.state[p] = {"step": step[0], **views}
-        return {"flat": flat, "step": step, "table": table, "device": dev, "sizes": sizes,
+        d = _lib.AdamWDesc()
+        d.state_bits = self._state_bits
+        second = "exp_avg_sq" if self._state_bits == 32 else "exp_avg_sqrt"
+        d.d_step, d.d_exp_avg, d.d_exp_avg_sq = step.data_ptr(), flat["exp_avg"].data_ptr(), flat[second].data_ptr()
+        if self._state_bits == 8:
+            d.d_exp_avg_scale = flat["exp_avg_scale"].data_ptr()
+            d.d_exp_avg_sq_scale = flat["exp_avg_sqrt_scale"].data_ptr()
+        return {"flat": flat, "step": step, "table": table, "desc": d, "device": dev, "sizes": sizes,
                 "strides": [p.stride() for p in params]}
 
     @staticmethod
@@ -154,78 +171,94 @@ class AdamW(torch.optim.Optimizer):
             group.update({k: v for k, v in saved.items() if k not in ("params", "strides")})
 
     # -- step ---------------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, closure=None):
+        for hook in (*_PRE_HOOKS.values(), *self._optimizer_step_pre_hooks.values()):
+            changed = hook(self, (self, closure), {})
+            if changed is not None:
+                closure = changed[0][1]
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
         for group, plan in zip(self.param_groups, self._plans):
             self._step_group(group, plan)
+        for hook in (*self._optimizer_step_post_hooks.values(), *_POST_HOOKS.values()):
+            hook(self, (self, closure), {})
         return loss
 
-    def _step_group(self, group, plan) -> None:
-        keep, chosen, kinds, ptrs = [], [], [], []
-        sizes, strides = plan["sizes"], plan["strides"]
-        for i, p in enumerate(group["params"]):
-            g = p.grad
+    # torch wraps an optimizer's step in a profiler range and calls the hooks there, 10 us of the host's time in a step
+    # whose launch takes 4; the hooks are called above instead
+    step.hooked = True
+
+    def _gather(self, group, plan):
+        """Parameters that take part in a step, their gradients in the parameters' order of memory, and their places."""
+        params, strides, sizes = group["params"], plan["strides"], plan["sizes"]
+        grads = [p.grad for p in params]
+        # whole lists at a time: a loop over the tensors costs the host twice as much
+        try:
+            ordinary = (list(map(_stride, grads)) == strides and list(map(_numel, grads)) == sizes
+                        and list(map(_stride, params)) == strides and list(map(_numel, params)) == sizes and 0 not in sizes)
+        except (TypeError, RuntimeError):   # a gradient that is None, or has no strides (sparse)
+            ordinary = False
+        if ordinary:
+            return params, grads, plan["table"].copy()
+        chosen, kept = [], []
+        for i, (p, g) in enumerate(zip(params, grads)):
             if g is None or sizes[i] == 0:
                 continue
-            s = strides[i]
-            if p.stride() != s or p.numel() != sizes[i]:
-                if p.numel() != sizes[i] or not _dense(p):
-                    raise ValueError("AdamW: a parameter has changed its size, or is no longer dense")
-                if self._state_bits == 8 or p.device != plan["device"]:
-                    raise ValueError("AdamW: a parameter has changed its memory format or device")
-                raise ValueError("AdamW: a parameter has changed its memory format")
-            if g.layout is not torch.strided:
+            if p.stride() != strides[i] or p.numel() != sizes[i] or p.device != plan["device"]:
+                raise ValueError("AdamW: a parameter has changed its size, memory format or device")
+            if g.layout is not _STRIDED:
                 raise ValueError("AdamW: sparse gradients are not supported")
-            if g.dtype not in _DTYPES:
-                g = g.float()
-            if g.stride() != s or g.numel() != sizes[i]:
-                g = torch.empty_strided(p.shape, s, dtype=g.dtype, device=g.device).copy_(g)
-                keep.append(g)
+            if g.stride() != strides[i] or g.numel() != sizes[i]:
+                g = torch.empty_strided(p.shape, strides[i], dtype=g.dtype, device=g.device).copy_(g.detach())
             chosen.append(i)
-            kinds.append((p.dtype, g.dtype))
-            ptrs.append((p.data_ptr(), g.data_ptr()))
-        if not chosen:
+            kept.append(g)
+        return [params[i] for i in chosen], kept, plan["table"][chosen]
+
+    def _step_group(self, group, plan) -> None:
+        params, grads, table = self._gather(group, plan)
+        if not params:
             return
-        dev = plan["device"]
-        table = plan["table"][chosen]
-        table[:, :2] = ptrs
-        d = _lib.AdamWDesc()
-        d.state_bits = self._state_bits
-        lr = group["lr"]
-        if isinstance(lr, torch.Tensor) and lr.is_cuda:
-            lr = lr.detach().to(device=dev, dtype=torch.float32)
-            keep.append(lr)
-            d.d_lr = lr.data_ptr()
-        else:
-            d.lr = float(lr)
+        kinds = list(zip(map(_dtype, params), map(_dtype, grads)))
+        distinct = set(kinds)
+        for pair in distinct:
+            if pair[0] not in _DTYPES:
+                raise ValueError(f"AdamW: parameters must be float32, float16 or bfloat16 (got {pair[0]})")
+        if any(pair[1] not in _DTYPES for pair in distinct):
+            grads = [g if g.dtype in _DTYPES else g.detach().float() for g in grads]
+            kinds = list(zip(map(_dtype, params), map(_dtype, grads)))
+            distinct = set(kinds)
+        table[:, 0] = list(map(_data_ptr, params))
+        table[:, 1] = list(map(_data_ptr, grads))
+        dev, flat, d = plan["device"], plan["flat"], plan["desc"]
         d.beta1, d.beta2 = group["betas"]
         d.eps, d.weight_decay = group["eps"], group["weight_decay"]
+        keep = []
+        lr = group["lr"]
+        if isinstance(lr, torch.Tensor) and lr.is_cuda:
+            keep.append(lr.detach().to(device=dev, dtype=torch.float32))
+            d.d_lr, d.lr = keep[-1].data_ptr(), 0.0
+        else:
+            d.d_lr, d.lr = None, float(lr)
+        d.d_grad_scale = d.d_found_inf = None
         for name in ("grad_scale", "found_inf"):
             t = getattr(self, name, None)
             if t is not None:
-                t = t.to(device=dev, dtype=torch.float32)
+                if t.device != dev or t.dtype is not torch.float32:
+                    t = t.to(device=dev, dtype=torch.float32)
                 keep.append(t)
                 setattr(d, "d_" + name, t.data_ptr())
-        flat = plan["flat"]
-        d.d_step, d.d_exp_avg = plan["step"].data_ptr(), flat["exp_avg"].data_ptr()
-        if self._state_bits == 8:
-            d.d_exp_avg_sq, d.d_exp_avg_scale = flat["exp_avg_sqrt"].data_ptr(), flat["exp_avg_scale"].data_ptr()
-            d.d_exp_avg_sq_scale = flat["exp_avg_sqrt_scale"].data_ptr()
-        else:
-            d.d_exp_avg_sq = flat["exp_avg_sq"].data_ptr()
-        distinct = list(dict.fromkeys(kinds))
+        launch = _lib.load().rexsc_adamw_step
         with _on(dev):
+            stream = _stream(dev)
             for j, kind in enumerate(distinct):
                 part = table if len(distinct) == 1 else np.ascontiguousarray(table[[k == kind for k in kinds]])
                 d.param_dtype, d.grad_dtype = _DTYPES[kind[0]], _DTYPES[kind[1]]
                 d.advance = j == len(distinct) - 1
-                _lib.check(_lib.load().rexsc_adamw_step(C.byref(d), part.ctypes.data, len(part), _stream(dev)),
-                           "rexsc_adamw_step")
-        del keep
+                rc = launch(C.byref(d), part.ctypes.data, len(part), stream)
+                if rc:
+                    _lib.check(rc, "rexsc_adamw_step")
 
 
 def _dense(t: torch.Tensor) -> bool:
