@@ -319,6 +319,10 @@ int rexsc_fxp_conv2d_fwd(const rexsc_fxp_conv_desc *desc, const void *d_act, con
  *   d_x, d_dy     fp32 / fp16 / bf16 (REXSC_*), rows `row_stride` elements apart, elements of a row next to each other
  *   d_out, d_dx, d_dw  dense; d_bias, d_db  [n]; each of its own REXSC_* type
  * Extents are 1 to 2^30.  Any of d_dx, d_dw, d_db may be null; d_x (d_w) is needed for d_dw (d_dx) only.
+ * rexsc_int8_linear_fwd: weights quantised before (serving).  rexsc_int8_linear_workspace_size is 0 where the call needs no
+ * scratch (a few tokens, which the product's kernel quantises by itself) and for sizes that the call refuses; d_workspace may
+ * be null then.  rexsc_int8_linear_train_fwd quantises both operands and leaves them to the caller for the backward pass;
+ * with d_w null, d_wq and d_w_scale are read instead (weights that are not trained).
  * `kernel`: REXSC_INT8_AUTO, or one of the two product kernels; results are identical.
  * rexsc_int8_status synchronises the stream and returns REXSC_E_DEVICE_TIMEOUT if a bounded device-side wait of an int8
  * product on the current device gave up since it was last asked (that call's outputs are incomplete), else REXSC_OK.
@@ -333,10 +337,14 @@ int rexsc_int8_unpack(const int8_t *d_data, int64_t rows, int64_t cols, int8_t *
 int rexsc_int8_matmul(const int8_t *d_a, const float *d_a_scale, const int8_t *d_b, const float *d_b_scale,
                       const void *d_bias, int32_t bias_dtype, int64_t m, int64_t n, int64_t k, void *d_out,
                       int32_t out_dtype, int32_t kernel, void *stream);
-size_t rexsc_int8_linear_workspace_size(int64_t m, int64_t k);
+size_t rexsc_int8_linear_workspace_size(int64_t m, int64_t n, int64_t k, int32_t kernel);
 int rexsc_int8_linear_fwd(const void *d_x, int32_t dtype, int64_t m, int64_t k, int64_t row_stride, const int8_t *d_w,
                           const float *d_w_scale, int64_t n, const void *d_bias, int32_t bias_dtype, void *d_out,
                           int32_t out_dtype, int32_t kernel, void *d_workspace, size_t workspace_bytes, void *stream);
+int rexsc_int8_linear_train_fwd(const void *d_x, int32_t dtype, int64_t m, int64_t k, int64_t x_stride, const void *d_w,
+                                int32_t w_dtype, int64_t n, int64_t w_stride, const void *d_bias, int32_t bias_dtype,
+                                int8_t *d_xq, float *d_x_scale, int8_t *d_wq, float *d_w_scale, void *d_out,
+                                int32_t out_dtype, int32_t kernel, void *stream);
 size_t rexsc_int8_linear_bwd_workspace_size(int64_t m, int64_t n, int32_t want_dx, int32_t want_dw, int32_t want_db);
 int rexsc_int8_linear_bwd(const void *d_dy, int32_t dtype, int64_t m, int64_t n, int64_t k, int64_t row_stride,
                           const int8_t *d_x, const float *d_x_scale, const int8_t *d_w, const float *d_w_scale, void *d_dx,

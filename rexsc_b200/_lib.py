@@ -84,9 +84,11 @@ SYMBOLS = {
     "rexsc_int8_pack": (C.c_int, [_vp, _i64, _i64, _i64, _vp, _vp]),
     "rexsc_int8_unpack": (C.c_int, [_vp, _i64, _i64, _vp, _vp]),
     "rexsc_int8_matmul": (C.c_int, [_vp] * 5 + [_i32] + [_i64] * 3 + [_vp, _i32, _i32, _vp]),
-    "rexsc_int8_linear_workspace_size": (_sz, [_i64, _i64]),
+    "rexsc_int8_linear_workspace_size": (_sz, [_i64, _i64, _i64, _i32]),
     "rexsc_int8_linear_fwd": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i32, _i32, _vp, _sz,
                                         _vp]),
+    "rexsc_int8_linear_train_fwd": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _i64, _i64, _vp, _i32, _vp, _vp, _vp,
+                                              _vp, _vp, _i32, _i32, _vp]),
     "rexsc_int8_linear_bwd_workspace_size": (_sz, [_i64, _i64, _i32, _i32, _i32]),
     "rexsc_int8_linear_bwd": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp,
                                         _i32, _i32, _vp, _sz, _vp]),

@@ -53,5 +53,10 @@ struct I8Product {
 };
 // kernel: REXSC_INT8_*.  after_quantize: the launch may begin while the previous one on the stream (which writes operand a) still runs
 int launch_i8_product(const I8Product &p, int kernel, bool after_quantize, cudaStream_t st);
+// two products that do not depend on one another, in one launch where both are small
+int launch_i8_products(const I8Product &p, const I8Product &q, int kernel, bool after_quantize, cudaStream_t st);
+// a few tokens that the product's kernel quantises by itself: x takes the place of p.a and p.row_scale
+bool i8_tokens_fit(long long m, long long n, long long k, int kernel);
+int launch_i8_tokens(const void *x, int dtype, long long stride, const I8Product &p, cudaStream_t st);
 
 } // namespace rexsc

@@ -9,12 +9,13 @@
 //                        the epilogue of a tile runs under the next one's products.
 //   product_split_kernel 128 columns of the output (lanes of TMEM) x 16 to 128 rows per CTA; the CTAs of a cluster split the
 //                        contraction and join their int32 sums through distributed shared memory (whole numbers: the
-//                        order does not matter).
+//                        order does not matter).  It takes two products in one launch (a layer's two gradients), and up
+//                        to 16 tokens as they are, which it quantises itself.
 // Every mbarrier wait is bounded; a CTA whose wait gives up raises the library's status word (rexsc_int8_status), stores
 // nothing more, waits for its copies in flight, frees its TMEM and leaves.
 #include <cuda.h>
 
-#include "int8.cuh"
+#include "int8_quant.cuh"
 
 namespace rexsc {
 
@@ -75,6 +76,7 @@ __device__ __forceinline__ void copy_tile_pair(uint32_t dst, const CUtensorMap *
 }
 __device__ __forceinline__ void cluster_sync()
 {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank()
@@ -391,61 +393,149 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
     }
 }
 
-struct SplitArgs {
+struct SplitProblem {
     I8Product p;
     long long tiles_j;  // blocks of 128 output columns
     int rows;           // output rows per CTA: 16, 32, 64 or 128
-    int split;          // CTAs of the cluster
     int k_blocks;
     int stages;
     int q_bytes;        // bytes of a stage's rows operand
     int tmem_cols;
     int store_bytes;
 };
+struct SplitArgs {
+    SplitProblem p[2];
+    unsigned first;     // CTAs of p[0]; the others work on p[1]
+    int split;          // CTAs of a cluster
+    const void *x;      // tokens in place of p[0]'s rows operand
+    long long x_stride;
+    int x_vec;          // its rows begin on 16 bytes
+};
 
 constexpr int kSplitThreads = 128;
 constexpr int kSplitMaxStages = 12;
 constexpr size_t kSplitSmemMost = 212 * 1024;
+constexpr int kTokenRows = 16;                      // most tokens that the kernel quantises by itself
+constexpr int kTokenBlockBytes = kTokenRows * 128;  // 128 columns of them
+constexpr int kTokenMaxBlocks = 32;                 // such blocks a CTA holds
 
-template <typename T>
-__device__ __forceinline__ void store4(T *dst, const float (&v)[4], int live, bool aligned)
+__device__ __forceinline__ void store1(void *out, int dtype, long long i, float v)
+{
+    if (dtype == REXSC_F32) static_cast<float *>(out)[i] = v;
+    else if (dtype == REXSC_F16) static_cast<__half *>(out)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(out)[i] = __float2bfloat16_rn(v);
+}
+__device__ __forceinline__ void store4(void *out, int dtype, long long i, const float (&v)[4], int live, bool aligned)
 {
     if (live >= 4 && aligned) {
-        if constexpr (sizeof(T) == 4)
-            *reinterpret_cast<float4 *>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+        if (dtype == REXSC_F32)
+            *reinterpret_cast<float4 *>(static_cast<float *>(out) + i) = make_float4(v[0], v[1], v[2], v[3]);
+        else if (dtype == REXSC_F16)
+            *reinterpret_cast<uint2 *>(static_cast<__half *>(out) + i) =
+                make_uint2(pack2(__float2half_rn(v[0]), __float2half_rn(v[1])), pack2(__float2half_rn(v[2]), __float2half_rn(v[3])));
         else
-            *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(round_to<T>(v[0]), round_to<T>(v[1])), pack2(round_to<T>(v[2]), round_to<T>(v[3])));
+            *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(out) + i) = make_uint2(
+                pack2(__float2bfloat16_rn(v[0]), __float2bfloat16_rn(v[1])), pack2(__float2bfloat16_rn(v[2]), __float2bfloat16_rn(v[3])));
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (i < live) dst[i] = round_to<T>(v[i]);
+        for (int k = 0; k < 4; k++)
+            if (k < live) store1(out, dtype, i + k, v[k]);
     }
 }
 
-template <typename T>
+// X: int8_t where the rows operand is a matrix of tiles; else the type of up to 16 tokens that every CTA quantises for itself,
+// its part of the contraction only: the CTAs of a cluster tell one another the largest magnitudes of their parts.
+template <typename X>
 __global__ void __launch_bounds__(kSplitThreads)
-product_split_kernel(const __grid_constant__ SplitArgs a)
+product_split_kernel(const __grid_constant__ SplitArgs args)
 {
+    constexpr bool kTokens = !std::is_same<X, int8_t>::value;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * kSplitMaxStages + 1];
     __shared__ uint32_t tmem_slot;
+    __shared__ uint32_t part_most[kTokenRows];
+    __shared__ float row_a[kTokenRows], row_inv[kTokenRows], row_s[kTokenRows];
     uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     const uint32_t bar0 = smem_addr(bars);
     auto full = [&](int s) { return bar0 + s * 8; };
     auto empty = [&](int s) { return bar0 + (kSplitMaxStages + s) * 8; };
     const uint32_t acc_full = bar0 + 2 * kSplitMaxStages * 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = a.split > 1 ? (int)cluster_rank() : 0;
-    const long long tile = blockIdx.x / a.split, tj = tile % a.tiles_j, ti = tile / a.tiles_j;
-    const int k0 = (int)((long long)rank * a.k_blocks / a.split), k1 = (int)((long long)(rank + 1) * a.k_blocks / a.split);
+    const int which = !kTokens && blockIdx.x >= args.first;
+    const SplitProblem &a = args.p[which];
+    const int split = args.split, rank = split > 1 ? (int)cluster_rank() : 0;
+    const unsigned tile = (blockIdx.x - (which ? args.first : 0)) / split;
+    const long long ti = tile / a.tiles_j, tj = tile - ti * a.tiles_j;
+    const int k0 = (int)((long long)rank * a.k_blocks / split), nk = (int)((long long)(rank + 1) * a.k_blocks / split) - k0;
     const long long row0 = ti * a.rows, col0 = tj * 128;
     const int rows = a.p.m - row0 < a.rows ? (int)(a.p.m - row0) : a.rows; // that exist
+    const uint32_t smem0 = smem_addr(smem), stage_bytes = kI8TileBytes + (kTokens ? 0 : a.q_bytes);
+    const uint32_t tokens0 = smem0 + a.stages * stage_bytes; // the quantised tokens, [128 columns][16][128 bytes]
+    const int early = nk < a.stages ? nk : a.stages;
 
+    const int8_t *pw = a.p.b.data + ((size_t)(tj * a.p.b.step_mn) + (size_t)(k0 * a.p.b.step_k)) * kI8TileBytes;
+    const size_t step_w = (size_t)a.p.b.step_k * kI8TileBytes;
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
         mbar_init(acc_full, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        // the weights depend neither on the tokens nor on the launch before, which quantises the rows: begin with them
+        for (int s = 0; s < early; s++) {
+            mbar_expect(full(s), stage_bytes);
+            copy_in(smem0 + s * stage_bytes, pw, kI8TileBytes, full(s));
+            pw += step_w;
+        }
     }
+    if constexpr (kTokens) {
+        const X *x = static_cast<const X *>(args.x);
+        // warps to a row: all four have the only token, two each of two, else every warp has rows of its own
+        const int team = rows == 1 ? 4 : rows == 2 ? 2 : 1, part = warp % team;
+        if (threadIdx.x < kTokenRows) part_most[threadIdx.x] = 0;
+        __syncthreads();
+        for (int r = warp / team; r < rows; r += 4 / team) {
+            uint32_t most = 0;
+            for (long long c = (long long)k0 * 128 + (part * 32 + lane) * 8; c < (long long)(k0 + nk) * 128; c += team * 256) {
+                Raw<X> raw;
+                load_raw(x + r * args.x_stride, c, a.p.k, args.x_vec, raw);
+                most_of(raw, most);
+            }
+            most = __reduce_max_sync(0xffffffffu, most_as_f32<X>(most));
+            if (lane == 0) atomicMax(&part_most[r], most);
+        }
+        if (split > 1) cluster_sync();
+        else __syncthreads();
+        if (threadIdx.x < kTokenRows) {
+            uint32_t most = 0;
+            for (int r = 0; r < split; r++) {
+                uint32_t v = part_most[threadIdx.x];
+                if (split > 1)
+                    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(map_rank(smem_addr(&part_most[threadIdx.x]), r)) : "memory");
+                most = max(most, v);
+            }
+            const bool fine = most < 0x7f800000u, live = fine && most != 0;
+            row_a[threadIdx.x] = live ? __uint_as_float(most) : 0.f;
+            row_inv[threadIdx.x] = live ? inverse_of(__uint_as_float(most)) : 0.f;
+            row_s[threadIdx.x] = fine ? __fdiv_rn(__uint_as_float(most), 127.f) : __uint_as_float(0x7fc00000u);
+        }
+        __syncthreads();
+        for (int r = warp / team; r < rows; r += 4 / team) {
+            const float most = row_a[r], inv = row_inv[r];
+            for (int c = (part * 32 + lane) * 8; c < nk * 128; c += team * 256) {
+                Raw<X> raw;
+                float f[8];
+                load_raw(x + r * args.x_stride, (long long)k0 * 128 + c, a.p.k, args.x_vec, raw);
+                widen(raw, f);
+                const uint2 q = most > 0.f ? quant8<sizeof(X) == 2>(f, most, inv) : make_uint2(0u, 0u);
+                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(tokens0 + (c >> 7) * kTokenBlockBytes + r * 128 +
+                                                                     ((((c >> 4) & 7) ^ (r & 7)) << 4) + (c & 8)),
+                             "r"(q.x), "r"(q.y) : "memory");
+            }
+        }
+        // what was written is visible to the tensor core's reads
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    // TMEM from here on: while a CTA holds some it waits for nobody but its own copies and products, so that whoever waits for
+    // TMEM on this SM (of whatever kernel) always gets it
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"((uint32_t)a.tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -454,44 +544,40 @@ product_split_kernel(const __grid_constant__ SplitArgs a)
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_slot;
-    const uint32_t stage_bytes = kI8TileBytes + a.q_bytes;
 
     if (warp == 0) {
         if (lane == 0) { // ---- copies
-            const int8_t *pw = a.p.b.data + (size_t)(tj * a.p.b.step_mn) * kI8TileBytes;
-            const int8_t *px = a.p.a.data + (size_t)((row0 >> 7) * a.p.a.step_mn) * kI8TileBytes + (a.p.a.mn_major ? 0 : (row0 & 127) * 128);
-            const int n = k1 - k0, early = n < a.stages ? n : a.stages;
-            auto copy_w = [&](int i) {
-                const int s = i % a.stages;
+            const int8_t *px = a.p.a.data + ((size_t)((row0 >> 7) * a.p.a.step_mn) + (size_t)(k0 * a.p.a.step_k)) * kI8TileBytes +
+                               (a.p.a.mn_major ? 0 : (row0 & 127) * 128);
+            const size_t step_x = (size_t)a.p.a.step_k * kI8TileBytes;
+            auto copy_x = [&](int s) {
+                if (!kTokens) copy_in(smem0 + s * stage_bytes + kI8TileBytes, px, a.q_bytes, full(s));
+                px += step_x;
+            };
+            if (!kTokens) wait_previous_launch();
+            for (int s = 0; s < early; s++) copy_x(s);
+            int s = 0, phase = 0, filled = early;
+            for (; filled < nk; filled++) {
+                if (!mbar_wait(empty(s), phase)) break;
                 mbar_expect(full(s), stage_bytes);
-                copy_in(smem_addr(smem) + s * stage_bytes, pw + (size_t)((k0 + i) * a.p.b.step_k) * kI8TileBytes, kI8TileBytes, full(s));
-            };
-            auto copy_x = [&](int i) {
-                const int s = i % a.stages;
-                copy_in(smem_addr(smem) + s * stage_bytes + kI8TileBytes, px + (size_t)((k0 + i) * a.p.a.step_k) * kI8TileBytes, a.q_bytes, full(s));
-            };
-            // the weights do not depend on the launch before, which quantises the rows
-            for (int i = 0; i < early; i++) copy_w(i);
-            wait_previous_launch();
-            for (int i = 0; i < early; i++) copy_x(i);
-            int i = early;
-            for (; i < n; i++) {
-                if (!mbar_wait(empty(i % a.stages), (i / a.stages - 1) & 1)) break;
-                copy_w(i);
-                copy_x(i);
+                copy_in(smem0 + s * stage_bytes, pw, kI8TileBytes, full(s));
+                pw += step_w;
+                copy_x(s);
+                if (++s == a.stages) s = 0, phase ^= 1;
             }
-            for (int j = i < a.stages ? 0 : i - a.stages; j < i; j++) mbar_wait(full(j % a.stages), (j / a.stages) & 1);
+            // nothing on its way when this CTA leaves: the last filling of every stage
+            for (int j = filled < a.stages ? 0 : filled - a.stages; j < filled; j++) mbar_wait(full(j % a.stages), (j / a.stages) & 1);
         }
     } else if (warp == 1) {
         if (lane == 0) { // ---- products: lanes are output columns, columns of TMEM output rows
             const uint32_t idesc = product_idesc(128, a.rows, a.p.b.mn_major, a.p.a.mn_major);
             const uint32_t adv_w = a.p.b.mn_major ? 4096 >> 4 : 32 >> 4, adv_x = a.p.a.mn_major ? 4096 >> 4 : 32 >> 4;
-            for (int i = 0; i < k1 - k0; i++) {
-                const int s = i % a.stages;
-                if (!mbar_wait(full(s), (i / a.stages) & 1)) break;
+            int s = 0, phase = 0;
+            for (int i = 0; i < nk; i++) {
+                if (!mbar_wait(full(s), phase)) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t sa = smem_addr(smem) + s * stage_bytes;
-                const uint64_t dw = tile_desc(sa), dx = tile_desc(sa + kI8TileBytes);
+                const uint32_t sa = smem0 + s * stage_bytes;
+                const uint64_t dw = tile_desc(sa), dx = tile_desc(kTokens ? tokens0 + i * kTokenBlockBytes : sa + kI8TileBytes);
 #pragma unroll
                 for (int q = 0; q < 4; q++)
                     asm volatile(
@@ -499,16 +585,17 @@ product_split_kernel(const __grid_constant__ SplitArgs a)
                         "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
                         "l"(dw + q * adv_w), "l"(dx + q * adv_x), "r"(idesc), "r"((uint32_t)(i | q)) : "memory");
                 asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(empty(s)) : "memory");
+                if (++s == a.stages) s = 0, phase ^= 1;
             }
             // (after a wait that gave up: of what was issued)
             asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(acc_full) : "memory");
         }
     }
     __syncwarp();
-    wait_previous_launch();
-    mbar_wait(acc_full, 0);
+    if (!kTokens) wait_previous_launch();
+    if (lane == 0) mbar_wait(acc_full, 0); // (one lane of a warp asks)
+    __syncwarp();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    T *out = static_cast<T *>(a.p.out);
     const uint32_t tmem_lane = tmem + ((uint32_t)(warp * 32) << 16);
     auto free_tmem = [&]() {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -518,7 +605,8 @@ product_split_kernel(const __grid_constant__ SplitArgs a)
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)a.tmem_cols) : "memory");
         }
     };
-    if (a.split == 1) {
+    auto scale_of = [&](int r) { return kTokens ? row_s[r] : a.p.row_scale[row0 + r]; };
+    if (split == 1) {
         const long long col = col0 + warp * 32 + lane;
         const bool live = col < a.p.n;
         const float cs = live && a.p.col_scale ? a.p.col_scale[col] : 1.f;
@@ -531,52 +619,50 @@ product_split_kernel(const __grid_constant__ SplitArgs a)
 #pragma unroll
                 for (int i = 0; i < 16; i++)
                     if (c + i < rows)
-                        out[(row0 + c + i) * a.p.out_stride + col] = round_to<T>(scaled(v[i], a.p.row_scale[row0 + c + i], cs, bias));
+                        store1(a.p.out, a.p.out_dtype, (row0 + c + i) * a.p.out_stride + col, scaled(v[i], scale_of(c + i), cs, bias));
             }
         }
         __syncwarp();
-    } else {
-        // sums to shared memory, [row][column]; every CTA of the cluster finishes some of the rows
-        int *red = reinterpret_cast<int *>(smem);
-        for (int c = 0; c < rows; c += 16) {
-            int v[16];
-            tmem_load16(tmem_lane + c, v);
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (c + i < rows) red[(c + i) * 128 + warp * 32 + lane] = v[i];
-        }
-        // TMEM is given back before the CTAs of the cluster wait for one another: a CTA that holds TMEM then waits for nobody
-        // but itself, and one that waits for TMEM (of whatever kernel shares the SM) always gets it
         free_tmem();
-        cluster_sync();
-        const long long col = col0 + lane * 4;
-        const int live = a.p.n - col < 4 ? (int)(a.p.n - col) : 4;
-        if (live > 0) {
-            float cs[4], bias[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                cs[i] = i < live && a.p.col_scale ? a.p.col_scale[col + i] : 1.f;
-                bias[i] = i < live && a.p.bias ? load_any(a.p.bias, a.p.bias_dtype, col + i) : 0.f;
-            }
-            for (int c = rank * 4 + warp; c < rows; c += 4 * a.split) {
-                int4 sum = make_int4(0, 0, 0, 0);
-                const uint32_t at = smem_addr(red + c * 128 + lane * 4);
-                for (int r = 0; r < a.split; r++) {
-                    int4 v;
-                    asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(map_rank(at, r)) : "memory");
-                    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-                }
-                const float rs = a.p.row_scale[row0 + c];
-                const float f[4] = {scaled(sum.x, rs, cs[0], bias[0]), scaled(sum.y, rs, cs[1], bias[1]),
-                                    scaled(sum.z, rs, cs[2], bias[2]), scaled(sum.w, rs, cs[3], bias[3])};
-                store4(out + (row0 + c) * a.p.out_stride + col, f, live, a.store_bytes >= 16);
-            }
-        }
-        __syncwarp();
-        cluster_sync(); // the others still read this CTA's sums
+        return;
     }
-    if (a.split == 1) free_tmem();
+    // sums to shared memory, [row][column]; every CTA of the cluster finishes some of the rows
+    int *red = reinterpret_cast<int *>(smem);
+    for (int c = 0; c < rows; c += 16) {
+        int v[16];
+        tmem_load16(tmem_lane + c, v);
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (c + i < rows) red[(c + i) * 128 + warp * 32 + lane] = v[i];
+    }
+    free_tmem();
+    cluster_sync();
+    const long long col = col0 + lane * 4;
+    const int live = a.p.n - col < 4 ? (int)(a.p.n - col) : 4;
+    if (live > 0) {
+        float cs[4], bias[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            cs[i] = i < live && a.p.col_scale ? a.p.col_scale[col + i] : 1.f;
+            bias[i] = i < live && a.p.bias ? load_any(a.p.bias, a.p.bias_dtype, col + i) : 0.f;
+        }
+        for (int c = rank * 4 + warp; c < rows; c += 4 * split) {
+            int4 sum = make_int4(0, 0, 0, 0);
+            const uint32_t at = smem_addr(red + c * 128 + lane * 4);
+            for (int r = 0; r < split; r++) {
+                int4 v;
+                asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(map_rank(at, r)) : "memory");
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+            const float rs = scale_of(c);
+            const float f[4] = {scaled(sum.x, rs, cs[0], bias[0]), scaled(sum.y, rs, cs[1], bias[1]),
+                                scaled(sum.z, rs, cs[2], bias[2]), scaled(sum.w, rs, cs[3], bias[3])};
+            store4(a.p.out, a.p.out_dtype, (row0 + c) * a.p.out_stride + col, f, live, a.store_bytes >= 16);
+        }
+    }
+    __syncwarp();
+    cluster_sync(); // the others still read this CTA's sums
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------
@@ -662,47 +748,103 @@ int launch_pair(const I8Product &p, bool overlap, cudaStream_t st)
     return launch_cluster(product_pair_kernel<T>, a, pairs * 2, 0, kPairThreads, kPairSmem, overlap, st, "product_pair_kernel");
 }
 
-template <typename T>
-int launch_split(const I8Product &p, bool overlap, cudaStream_t st)
-{
-    SplitArgs a;
-    a.p = p;
-    a.tiles_j = (p.n + 127) / 128;
-    a.k_blocks = (int)i8_tiles(p.k);
-    a.rows = p.a.mn_major || p.m > 64 ? 128 : p.m > 32 ? 64 : p.m > 16 ? 32 : 16;
-    const long long tiles = a.tiles_j * ((p.m + a.rows - 1) / a.rows);
-    a.split = 1;
-    while (a.split < 8 && a.split * 2 <= a.k_blocks && tiles * a.split * 2 <= 296) a.split *= 2;
-    a.q_bytes = p.a.mn_major ? kI8TileBytes : a.rows * 128;
-    const int stage = kI8TileBytes + a.q_bytes, most = (int)(kSplitSmemMost - 1024) / stage;
-    const int steps = (a.k_blocks + a.split - 1) / a.split;
-    a.stages = steps < kSplitMaxStages ? steps : kSplitMaxStages;
-    if (a.stages > most) a.stages = most;
-    a.tmem_cols = a.rows < 32 ? 32 : a.rows;
-    a.store_bytes = store_alignment(p);
-    size_t smem = (size_t)a.stages * stage;
-    if (a.split > 1 && smem < (size_t)a.rows * 512) smem = (size_t)a.rows * 512;
-    return launch_cluster(product_split_kernel<T>, a, tiles * a.split, a.split, kSplitThreads, smem + 1024, overlap, st,
-                          "product_split_kernel");
-}
-
-template <typename T>
-int launch_product(const I8Product &p, int kernel, bool overlap, cudaStream_t st)
+// ---- which kernel, and its shape
+bool use_pairs(const I8Product &p, int kernel)
 {
     const long long tiles = ((p.m + 255) / 256) * ((p.n + 255) / 256);
-    const bool pair = kernel == REXSC_INT8_PAIR || (kernel == REXSC_INT8_AUTO && p.m > 128 && tiles >= 37);
-    return pair ? launch_pair<T>(p, overlap, st) : launch_split<T>(p, overlap, st);
+    return kernel == REXSC_INT8_PAIR || (kernel == REXSC_INT8_AUTO && p.m > 128 && tiles >= 37);
+}
+
+long long split_shape(SplitProblem *a, const I8Product &p)
+{
+    a->p = p;
+    a->tiles_j = (p.n + 127) / 128;
+    a->k_blocks = (int)i8_tiles(p.k);
+    a->rows = p.a.mn_major || p.m > 64 ? 128 : p.m > 32 ? 64 : p.m > 16 ? 32 : 16;
+    a->q_bytes = p.a.mn_major ? kI8TileBytes : a->rows * 128;
+    a->tmem_cols = a->rows < 32 ? 32 : a->rows;
+    a->store_bytes = store_alignment(p);
+    return a->tiles_j * ((p.m + a->rows - 1) / a->rows);
+}
+
+// CTAs that share a contraction: as many as leave each a step of 128 and the GPU two CTAs an SM
+int split_of(long long tiles, int k_blocks)
+{
+    int split = 1;
+    while (split < 8 && split * 2 <= k_blocks && tiles * split * 2 <= 2 * 148) split *= 2;
+    return split;
+}
+
+// stages of a CTA, and the shared memory that it needs
+size_t split_stages(SplitProblem *a, int split, bool tokens)
+{
+    const int steps = (a->k_blocks + split - 1) / split, fixed = tokens ? steps * kTokenBlockBytes : 0;
+    const int stage = kI8TileBytes + (tokens ? 0 : a->q_bytes), most = ((int)kSplitSmemMost - 1024 - fixed) / stage;
+    a->stages = steps < kSplitMaxStages ? steps : kSplitMaxStages;
+    if (a->stages > most) a->stages = most;
+    size_t smem = (size_t)a->stages * stage + fixed;
+    if (split > 1 && smem < (size_t)a->rows * 512) smem = (size_t)a->rows * 512;
+    return smem + 1024;
+}
+
+int launch_split(const I8Product &p, const I8Product *second, bool overlap, cudaStream_t st)
+{
+    SplitArgs a = {};
+    const long long tiles = split_shape(&a.p[0], p), more = second ? split_shape(&a.p[1], *second) : 0;
+    int k_blocks = a.p[0].k_blocks;
+    if (second && a.p[1].k_blocks < k_blocks) k_blocks = a.p[1].k_blocks;
+    a.split = split_of(tiles + more, k_blocks);
+    size_t smem = split_stages(&a.p[0], a.split, false);
+    if (second) {
+        const size_t other = split_stages(&a.p[1], a.split, false);
+        if (other > smem) smem = other;
+    }
+    if ((tiles + more) * a.split > 0x7fffffffll) return REXSC_E_UNSUPPORTED;
+    a.first = (unsigned)(tiles * a.split);
+    return launch_cluster(product_split_kernel<int8_t>, a, (tiles + more) * a.split, a.split, kSplitThreads, smem, overlap, st,
+                          "product_split_kernel");
 }
 
 } // namespace
 
 int launch_i8_product(const I8Product &p, int kernel, bool after_quantize, cudaStream_t st)
 {
+    if (!use_pairs(p, kernel)) return launch_split(p, nullptr, after_quantize, st);
     switch (p.out_dtype) {
-    case REXSC_F32: return launch_product<float>(p, kernel, after_quantize, st);
-    case REXSC_F16: return launch_product<__half>(p, kernel, after_quantize, st);
-    default: return launch_product<__nv_bfloat16>(p, kernel, after_quantize, st);
+    case REXSC_F32: return launch_pair<float>(p, after_quantize, st);
+    case REXSC_F16: return launch_pair<__half>(p, after_quantize, st);
+    default: return launch_pair<__nv_bfloat16>(p, after_quantize, st);
     }
+}
+
+int launch_i8_products(const I8Product &p, const I8Product &q, int kernel, bool after_quantize, cudaStream_t st)
+{
+    if (!use_pairs(p, kernel) && !use_pairs(q, kernel)) return launch_split(p, &q, after_quantize, st);
+    const int rc = launch_i8_product(p, kernel, after_quantize, st);
+    return rc == REXSC_OK ? launch_i8_product(q, kernel, true, st) : rc;
+}
+
+bool i8_tokens_fit(long long m, long long n, long long k, int kernel)
+{
+    if (m > kTokenRows || kernel == REXSC_INT8_PAIR) return false;
+    const long long k_blocks = i8_tiles(k);
+    const int split = split_of((n + 127) / 128, (int)k_blocks);
+    return (k_blocks + split - 1) / split <= kTokenMaxBlocks;
+}
+
+int launch_i8_tokens(const void *x, int dtype, long long stride, const I8Product &p, cudaStream_t st)
+{
+    SplitArgs a = {};
+    const long long tiles = split_shape(&a.p[0], p);
+    a.split = split_of(tiles, a.p[0].k_blocks);
+    const size_t smem = split_stages(&a.p[0], a.split, true);
+    if (tiles * a.split > 0x7fffffffll) return REXSC_E_UNSUPPORTED;
+    a.first = (unsigned)(tiles * a.split);
+    a.x = x;
+    a.x_stride = stride;
+    a.x_vec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(stride * (long long)dtype_bytes(dtype))) & 15) == 0;
+    const auto kernel = dtype == REXSC_F32 ? product_split_kernel<float> : dtype == REXSC_F16 ? product_split_kernel<__half> : product_split_kernel<__nv_bfloat16>;
+    return launch_cluster(kernel, a, tiles * a.split, a.split, kSplitThreads, smem, false, st, "product_split_kernel");
 }
 
 } // namespace rexsc

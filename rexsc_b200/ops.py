@@ -806,27 +806,68 @@ def int8_matmul(a: Int8Matrix, b: Int8Matrix, bias: torch.Tensor = None, dtype: 
         return _int8_matmul(a, b, bias, dtype, what)
 
 
+@functools.lru_cache(maxsize=1024)
+def _int8_scratch(m: int, n: int, k: int, kernel: int) -> int:
+    return _lib.load().rexsc_int8_linear_workspace_size(m, n, k, kernel)
+
+
+@functools.lru_cache(maxsize=1024)
+def _int8_bwd_scratch(m: int, n: int, dx: bool, dw: bool, db: bool) -> int:
+    return _lib.load().rexsc_int8_linear_bwd_workspace_size(m, n, dx, dw, db)
+
+
+def _tile_bytes(rows: int, cols: int) -> int:
+    return -(-rows // 128) * -(-cols // 128) * 16384
+
+
 class _Int8Linear(torch.autograd.Function):
     """y = x w^T + bias with both operands in 8-bit integers; the gradients are products of 8-bit integers too."""
 
     @staticmethod
     def forward(ctx, x, weight, prepared, bias):
-        dev, n = x.device, (prepared or weight).shape[0]
-        x2 = _rows_of(x, x.shape[-1])
-        ctx.lead, ctx.dtypes = x.shape[:-1], (x.dtype, None if weight is None else weight.dtype,
-                                              None if bias is None else bias.dtype)
-        ctx.kernel = _int8_kernel()
-        if x2.shape[0] == 0:
-            ctx.sizes = (0, n, x.shape[-1])
+        dev = x.device
+        n, k = (weight if prepared is None else prepared).shape
+        xt = x.dtype
+        x2 = _rows_of(x, k)
+        m = x2.shape[0]
+        ctx.lead = x.shape[:-1]
+        ctx.dtypes = xt, None if weight is None else weight.dtype, None if bias is None else bias.dtype
+        ctx.sizes = m, n, k
+        if m == 0:
             return x2.new_empty((*ctx.lead, n))
+        ctx.kernel = kernel = _int8_kernel()
+        want_x, want_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         with _on(dev):
-            w = prepared if prepared is not None else _int8_quantize(_rows_of(weight, weight.shape[1]), "int8_linear")
-            q = _int8_quantize(x2, "int8_linear")
-            y = _int8_matmul(q, w, bias, x2.dtype, "int8_linear")
-        ctx.sizes = (q.rows, n, q.cols)
-        ctx.save_for_backward(*((q.data, q.scale) if ctx.needs_input_grad[1] else (None, q.scale)),
-                              *((w.data, w.scale) if ctx.needs_input_grad[0] else (None, None)))
-        return y.view(*ctx.lead, n)
+            # both quantised operands with their scales; one buffer where the backward pass needs both
+            at_w = _tile_bytes(m, k) + -(-m // 64) * 256
+            nbytes = at_w + (_tile_bytes(n, k) + -(-n // 64) * 256 if prepared is None else 0)
+            buf = torch.empty(nbytes, dtype=torch.int8, device=dev)
+            base = buf.data_ptr()
+            xs = base + _tile_bytes(m, k)
+            if prepared is None:
+                w2 = _rows_of(weight, k)
+                wd, w_ptr, w_dtype, w_stride = base + at_w, w2.data_ptr(), _DTYPES[w2.dtype], w2.stride(0)
+                ws = wd + _tile_bytes(n, k)
+            else:
+                wd, ws, w_ptr, w_dtype, w_stride = prepared.data.data_ptr(), prepared.scale.data_ptr(), 0, 0, 0
+            keep, bias_ptr, bias_dtype = _int8_bias(bias, n, dev, "int8_linear")
+            code = _DTYPES[x2.dtype]
+            y = torch.empty((m, n), dtype=x2.dtype, device=dev)
+            rc = _lib.load().rexsc_int8_linear_train_fwd(x2.data_ptr(), code, m, k, x2.stride(0), w_ptr, w_dtype, n, w_stride,
+                                                         bias_ptr, bias_dtype, base, xs, wd, ws, y.data_ptr(), code, kernel,
+                                                         _stream(dev))
+            if rc:
+                _lib.check(rc, "rexsc_int8_linear_train_fwd")
+            del keep
+            if prepared is not None:
+                kept = (None, prepared.data, prepared.scale)
+            elif want_x and not want_w:     # the activations are not needed again: only the weights stay
+                kept = (buf[at_w:].clone(), None, None)
+            else:
+                kept = (buf, None, None)
+        ctx.save_for_backward(*kept)
+        ctx.at_w = 0 if want_x and not want_w else at_w
+        return y if len(ctx.lead) == 1 else y.view(*ctx.lead, n)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -835,27 +876,40 @@ class _Int8Linear(torch.autograd.Function):
         want_dx, want_dw, _, want_db = ctx.needs_input_grad
         xt, wt, bt = ctx.dtypes
         dev = dy.device
+        if m == 0:
+            zeros = lambda want, shape, t: torch.zeros(shape, dtype=t, device=dev) if want else None
+            return zeros(want_dx, (*ctx.lead, k), xt), zeros(want_dw, (n, k), wt), None, zeros(want_db, (n,), bt)
         with _on(dev):
-            kept = lambda t: t if t in _DTYPES else torch.float32
-            if m == 0:
-                zeros = lambda want, shape, t: torch.zeros(shape, dtype=t, device=dev) if want else None
-                return zeros(want_dx, (*ctx.lead, k), xt), zeros(want_dw, (n, k), wt), None, zeros(want_db, (n,), bt)
-            xd, xs, wd, ws = ctx.saved_tensors
-            lib = _lib.load()
+            buf, wdata, wscale = ctx.saved_tensors
+            xd = xs = wd = ws = 0
+            if buf is not None:
+                base = buf.data_ptr()
+                xd, xs = base, base + _tile_bytes(m, k)
+                wd = base + ctx.at_w
+                ws = wd + _tile_bytes(n, k)
+            if wdata is not None:
+                wd, ws = wdata.data_ptr(), wscale.data_ptr()
             g = _rows_of(dy, n)
-            dx = torch.empty((m, k), dtype=kept(xt), device=dev) if want_dx else None
-            dw = torch.empty((n, k), dtype=kept(wt), device=dev) if want_dw else None
-            db = torch.empty((n,), dtype=kept(bt), device=dev) if want_db else None
-            nbytes = lib.rexsc_int8_linear_bwd_workspace_size(m, n, want_dx, want_dw, want_db)
+            dx = torch.empty((m, k), dtype=xt if xt in _DTYPES else torch.float32, device=dev) if want_dx else None
+            dw = torch.empty((n, k), dtype=wt if wt in _DTYPES else torch.float32, device=dev) if want_dw else None
+            db = torch.empty((n,), dtype=bt if bt in _DTYPES else torch.float32, device=dev) if want_db else None
+            nbytes = _int8_bwd_scratch(m, n, want_dx, want_dw, want_db)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            ptr = lambda t: 0 if t is None else _ptr(t)
+            ptr = lambda t: 0 if t is None else t.data_ptr()
             code = lambda t: 0 if t is None else _DTYPES[t.dtype]
-            rc = lib.rexsc_int8_linear_bwd(_ptr(g), _DTYPES[g.dtype], m, n, k, g.stride(0), ptr(xd), ptr(xs), ptr(wd), ptr(ws),
-                                           ptr(dx), code(dx), ptr(dw), code(dw), ptr(db), code(db), ctx.kernel,
-                                           _ptr(scratch), nbytes, _stream(dev))
-            _lib.check(rc, "rexsc_int8_linear_bwd")
-            return (None if dx is None else dx.view(*ctx.lead, k).to(xt), None if dw is None else dw.to(wt), None,
-                    None if db is None else db.to(bt))
+            rc = _lib.load().rexsc_int8_linear_bwd(g.data_ptr(), _DTYPES[g.dtype], m, n, k, g.stride(0), xd, xs, wd, ws,
+                                                   ptr(dx), code(dx), ptr(dw), code(dw), ptr(db), code(db), ctx.kernel,
+                                                   scratch.data_ptr(), nbytes, _stream(dev))
+            if rc:
+                _lib.check(rc, "rexsc_int8_linear_bwd")
+            if dx is not None:
+                dx = dx if len(ctx.lead) == 1 else dx.view(*ctx.lead, k)
+                dx = dx if dx.dtype == xt else dx.to(xt)
+            if dw is not None and dw.dtype != wt:
+                dw = dw.to(wt)
+            if db is not None and db.dtype != bt:
+                db = db.to(bt)
+            return dx, dw, None, db
 
 
 @_traced
@@ -875,49 +929,49 @@ def int8_linear(x: torch.Tensor, weight, bias: torch.Tensor = None) -> torch.Ten
     Both directions can be captured into a CUDA graph; every call has scratch of its own.  As with any op of torch, drop all
     eager graphs of the same leaves (outputs that still hold one) before capturing a backward pass: torch's engine would wait
     on the stream of their leaf nodes, which ends the capture, or the process, with an error."""
-    what = "int8_linear"
-    _require_cuda(x, what)
-    prepared = isinstance(weight, Int8Matrix)
-    if not prepared:
-        _require_cuda(weight, what)
+    prepared = type(weight) is Int8Matrix
+    if prepared:
+        n, k, dev = weight.rows, weight.cols, weight.data.device
+    else:
+        _require_cuda(weight, "int8_linear")
         if weight.dim() != 2 or not weight.is_floating_point():
-            raise ValueError(f"{what}: expected a floating-point weight [n, k] or an Int8Matrix")
-    n, k = weight.shape
-    if x.dim() < 1 or x.shape[-1] != k or n == 0 or k == 0 or not x.is_floating_point():
-        raise ValueError(f"{what}: expected floating-point x [..., {k}] for weights [{n}, {k}], neither of them 0")
-    if weight.device != x.device:
-        raise ValueError(f"{what}: x is on {x.device}, the weights are on {weight.device}")
+            raise ValueError("int8_linear: expected a floating-point weight [n, k] or an Int8Matrix")
+        (n, k), dev = weight.shape, weight.device
+    if x.device != dev or x.dim() < 1 or x.size(-1) != k or n == 0 or k == 0 or not x.is_floating_point():
+        _require_cuda(x, "int8_linear")
+        if x.device != dev:
+            raise ValueError(f"int8_linear: x is on {x.device}, the weights are on {dev}")
+        raise ValueError(f"int8_linear: expected floating-point x [..., {k}] for weights [{n}, {k}], neither of them 0")
     if k > _lib.INT8_MAX_DOT:
-        raise ValueError(f"{what}: sums of more than {_lib.INT8_MAX_DOT} products are not supported (k = {k})")
+        raise ValueError(f"int8_linear: sums of more than {_lib.INT8_MAX_DOT} products are not supported (k = {k})")
     if torch.is_grad_enabled() and (x.requires_grad or (not prepared and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        _int8_bias(bias, n, x.device, what)
         if x.requires_grad and n > _lib.INT8_MAX_DOT:
-            raise ValueError(f"{what}: the gradient of x sums over {n} output channels, at most {_lib.INT8_MAX_DOT}")
+            raise ValueError(f"int8_linear: the gradient of x sums over {n} output channels, at most {_lib.INT8_MAX_DOT}")
         if not prepared and weight.requires_grad and x.numel() // k > _lib.INT8_MAX_DOT:
-            raise ValueError(f"{what}: the weight's gradient sums over {x.numel() // k} tokens, at most {_lib.INT8_MAX_DOT}")
+            raise ValueError(f"int8_linear: the weight's gradient sums over {x.numel() // k} tokens, at most "
+                             f"{_lib.INT8_MAX_DOT}")
         return _Int8Linear.apply(x, None if prepared else weight, weight if prepared else None, bias)
-    dev = x.device
-    lib = _lib.load()
     with _on(dev):
-        x2 = _rows_of(x, k)
-        m = x2.shape[0]
-        keep, bias_ptr, bias_dtype = _int8_bias(bias, n, dev, what)
-        out = torch.empty((m, n), dtype=x2.dtype, device=dev)
+        ordinary = x.dim() == 2 and x.dtype in _DTYPES and x.stride(1) == 1
+        x2 = x if ordinary else _rows_of(x, k)
+        m = x2.size(0)
+        keep, bias_ptr, bias_dtype = (None, 0, 0) if bias is None else _int8_bias(bias, n, dev, "int8_linear")
+        out = x2.new_empty((m, n))
         if m:
-            w = weight if prepared else _int8_quantize(_rows_of(weight, k), what)
-            nbytes = lib.rexsc_int8_linear_workspace_size(m, k)
-            if nbytes == 0:
-                raise ValueError(f"{what}: unsupported size {m} x {k}")
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            rc = lib.rexsc_int8_linear_fwd(_ptr(x2), _DTYPES[x2.dtype], m, k, x2.stride(0), _ptr(w.data), _ptr(w.scale), n,
-                                           bias_ptr, bias_dtype, _ptr(out), _DTYPES[x2.dtype], _int8_kernel(),
-                                           _ptr(scratch), nbytes, _stream(dev))
-            _lib.check(rc, "rexsc_int8_linear_fwd")
+            w = weight if prepared else _int8_quantize(_rows_of(weight, k), "int8_linear")
+            kernel, code = _int8_kernel(), _DTYPES[x2.dtype]
+            nbytes = _int8_scratch(m, n, k, kernel)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+            rc = _lib.load().rexsc_int8_linear_fwd(x2.data_ptr(), code, m, k, x2.stride(0), w.data.data_ptr(),
+                                                   w.scale.data_ptr(), n, bias_ptr, bias_dtype, out.data_ptr(), code, kernel,
+                                                   scratch.data_ptr() if nbytes else 0, nbytes, _stream(dev))
+            if rc:
+                _lib.check(rc, "rexsc_int8_linear_fwd")
             if _DEBUG:
-                _lib.check(lib.rexsc_int8_status(_stream(dev)), "rexsc_int8_linear_fwd (device status)")
+                _lib.check(int8_status(dev), "rexsc_int8_linear_fwd (device status)")
     del keep
-    return out.view(*x.shape[:-1], n)
+    return out if ordinary else out.view(*x.shape[:-1], n)
 
 
 def int8_status(device=None) -> int:

@@ -19,8 +19,11 @@ def test_sizes_of_8_bit_matrices(lib):
         assert lib.rexsc_int8_data_size(rows, cols) == tiles * tile
     for rows, cols in [(0, 1), (1, 0), (-1, 5), ((1 << 30) + 1, 1)]:
         assert lib.rexsc_int8_data_size(rows, cols) == 0
-    assert lib.rexsc_int8_linear_workspace_size(1, 4096) == 256 + 32 * tile
-    assert lib.rexsc_int8_linear_workspace_size(1, 131072) == 0
+    assert lib.rexsc_int8_linear_workspace_size(17, 4096, 4096, 0) == 256 + 32 * tile
+    assert lib.rexsc_int8_linear_workspace_size(16, 4096, 4096, 0) == 0          # the product's kernel quantises a few tokens
+    assert lib.rexsc_int8_linear_workspace_size(16, 4096, 4096, 2) == 256 + 32 * tile
+    assert lib.rexsc_int8_linear_workspace_size(1, 8, 131071, 0) == 256 + 1024 * tile   # too long for that
+    assert lib.rexsc_int8_linear_workspace_size(17, 4096, 131072, 0) == 0
     both = lib.rexsc_int8_linear_bwd_workspace_size(300, 500, 1, 1, 1)
     assert both > 2 * 3 * 4 * tile
     assert lib.rexsc_int8_linear_bwd_workspace_size(300, 500, 1, 0, 0) < both
@@ -45,8 +48,14 @@ def test_int8_entry_points_refuse_bad_arguments(lib):
     assert mm(p, None, p, p, None, 0, 4, 4, 128, p, 0, 0, None) == -1
     assert mm(off, p, p, p, None, 0, 4, 4, 128, p, 0, 0, None) == -1
     fwd = lib.rexsc_int8_linear_fwd
-    assert fwd(p, 0, 4, 128, 128, p, p, 8, None, 0, p, 0, 0, None, 0, None) == -3
-    assert fwd(p, 0, 4, 128, 128, p, p, 8, None, 0, p, 0, 0, p, 256, None) == -3
+    assert fwd(p, 0, 40, 128, 128, p, p, 8, None, 0, p, 0, 0, None, 0, None) == -3
+    assert fwd(p, 0, 40, 128, 128, p, p, 8, None, 0, p, 0, 0, p, 256, None) == -3
+    assert fwd(p, 0, 40, 128, 128, off, p, 8, None, 0, p, 0, 0, p, 1 << 30, None) == -1
+    train = lib.rexsc_int8_linear_train_fwd
+    assert train(p, 0, 4, 128, 128, p, 0, 8, 128, None, 0, off, p, p, p, p, 0, 0, None) == -1
+    assert train(p, 0, 4, 128, 128, p, 7, 8, 128, None, 0, p, p, p, p, p, 0, 0, None) == -1
+    assert train(p, 0, 4, 128, 128, p, 0, 8, 128, None, 0, p, None, p, p, p, 0, 0, None) == -1
+    assert train(p, 0, 4, 131072, 131072, p, 0, 8, 131072, None, 0, p, p, p, p, p, 0, 0, None) == -4
     assert fwd(p, 0, 4, 131072, 131072, p, p, 8, None, 0, p, 0, 0, p, 1 << 40, None) == -4
     bwd = lib.rexsc_int8_linear_bwd
     assert bwd(p, 0, 4, 8, 128, 8, p, p, p, p, None, 0, None, 0, None, 0, 0, p, 1 << 30, None) == -1   # nothing wanted
