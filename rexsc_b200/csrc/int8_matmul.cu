@@ -167,45 +167,40 @@ constexpr int kPairStages = 6;
 constexpr int kPairStageBytes = 2 * kI8TileBytes;
 constexpr int kPairThreads = 192;     // producer, products, four warps for the epilogue
 constexpr int kGroupTiles = 8;        // output tile rows that share the columns' operand while it is in L2
-constexpr size_t kPairSmem = kPairStages * kPairStageBytes + 1024 + 2 * 256 * 2 * sizeof(float) + 256;
+constexpr int kPairTurnFloats = 32 * 33; // a warp's 32 x 32 outputs on their way to whole rows
+constexpr size_t kPairSmem = kPairStages * kPairStageBytes + 1024 + (2 * 256 * 2 + 4 * kPairTurnFloats) * sizeof(float) + 256;
 
-// one lane's 32 neighbouring columns of a row
+// one lane's 32 neighbouring columns of a row, which begin on 16 or 32 bytes
 template <typename T>
-__device__ __forceinline__ void store_row(T *dst, const float (&v)[32], int live, int store_bytes)
+__device__ __forceinline__ void store_row(T *dst, const float (&v)[32], int store_bytes)
 {
-    if (live >= 32 && store_bytes >= 16) {
-        if constexpr (sizeof(T) == 4) {
-            if (store_bytes >= 32) {
+    if constexpr (sizeof(T) == 4) {
+        if (store_bytes >= 32) {
 #pragma unroll
-                for (int i = 0; i < 32; i += 8)
-                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + i), "f"(v[i]),
-                                 "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]),
-                                 "f"(v[i + 7]) : "memory");
-            } else {
-#pragma unroll
-                for (int i = 0; i < 32; i += 4)
-                    *reinterpret_cast<float4 *>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-            }
+            for (int i = 0; i < 32; i += 8)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + i), "f"(v[i]),
+                             "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3]), "f"(v[i + 4]), "f"(v[i + 5]), "f"(v[i + 6]),
+                             "f"(v[i + 7]) : "memory");
         } else {
-            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++) w[i] = pack2(round_to<T>(v[2 * i]), round_to<T>(v[2 * i + 1]));
-            if (store_bytes >= 32) {
-#pragma unroll
-                for (int i = 0; i < 16; i += 8)
-                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 2 * i), "r"(w[i]),
-                                 "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]),
-                                 "r"(w[i + 7]) : "memory");
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *reinterpret_cast<uint4 *>(dst + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-            }
+            for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<float4 *>(dst + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         }
     } else {
+        uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 32; i++)
-            if (i < live) dst[i] = round_to<T>(v[i]);
+        for (int i = 0; i < 16; i++) w[i] = pack2(round_to<T>(v[2 * i]), round_to<T>(v[2 * i + 1]));
+        if (store_bytes >= 32) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 2 * i), "r"(w[i]),
+                             "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]),
+                             "r"(w[i + 7]) : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<uint4 *>(dst + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        }
     }
 }
 
@@ -225,7 +220,8 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     float *col_s = reinterpret_cast<float *>(smem + kPairStages * kPairStageBytes); // [buffer][scale, bias][256]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(col_s + 2 * 2 * 256);
+    float *turn_s = col_s + 2 * 2 * 256;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(turn_s + 4 * kPairTurnFloats);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kPairStages + 5);
     const uint32_t bar0 = smem_addr(bars);
     auto full = [&](int s) { return bar0 + s * 8; };
@@ -373,9 +369,20 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
                     f[i] = scaled(v[i], rs, s4.x, b4.x), f[i + 1] = scaled(v[i + 1], rs, s4.y, b4.y);
                     f[i + 2] = scaled(v[i + 2], rs, s4.z, b4.z), f[i + 3] = scaled(v[i + 3], rs, s4.w, b4.w);
                 }
-                if (row < a.p.m) {
-                    const long long left = a.p.n - (col0 + c);
-                    store_row(out + row * a.p.out_stride + col0 + c, f, left < 32 ? (int)left : 32, a.store_bytes);
+                const long long left = a.p.n - (col0 + c);
+                if (left >= 32 && a.store_bytes >= 16) { // a lane's columns are whole vectors
+                    if (row < a.p.m) store_row(out + row * a.p.out_stride + col0 + c, f, a.store_bytes);
+                } else { // turned over in shared memory, so that a warp stores 32 neighbours of a row at a time
+                    float *mine = turn_s + quad * kPairTurnFloats;
+#pragma unroll
+                    for (int i = 0; i < 32; i++) mine[lane * 33 + i] = f[i];
+                    __syncwarp();
+                    const long long top = row - lane; // the warp's first row
+                    const int rows = a.p.m - top < 32 ? (int)(a.p.m - top) : 32;
+                    T *to = out + top * a.p.out_stride + col0 + c + lane;
+                    if (lane < left)
+#pragma unroll 8
+                        for (int i = 0; i < rows; i++, to += a.p.out_stride) *to = round_to<T>(mine[i * 33 + lane]);
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -410,6 +417,7 @@ struct SplitArgs {
     const void *x;      // tokens in place of p[0]'s rows operand
     long long x_stride;
     int x_vec;          // its rows begin on 16 bytes
+    int whole_rows;     // every CTA reads whole rows for their largest magnitudes
 };
 
 constexpr int kSplitThreads = 128;
@@ -418,6 +426,8 @@ constexpr size_t kSplitSmemMost = 212 * 1024;
 constexpr int kTokenRows = 16;                      // most tokens that the kernel quantises by itself
 constexpr int kTokenBlockBytes = kTokenRows * 128;  // 128 columns of them
 constexpr int kTokenMaxBlocks = 32;                 // such blocks a CTA holds
+constexpr int kTokenMaxValues = 8192;               // values a CTA quantises at the most: with more of them a launch of its own
+                                                    // is sooner done (13 x 2051 fp16 on 5003 channels: 23 us here, 9 us so)
 
 __device__ __forceinline__ void store1(void *out, int dtype, long long i, float v)
 {
@@ -486,46 +496,73 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
             pw += step_w;
         }
     }
+    // TMEM is taken once the CTAs of the cluster need nothing more from one another until it has been given back: a CTA that
+    // holds some waits for nobody but its own copies and products, so that whoever waits for TMEM on this SM (of whatever
+    // kernel) always gets it
+    auto take_tmem = [&]() {
+        if (warp == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"((uint32_t)a.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    };
+    __syncwarp();
     if constexpr (kTokens) {
         const X *x = static_cast<const X *>(args.x);
-        // warps to a row: all four have the only token, two each of two, else every warp has rows of its own
-        const int team = rows == 1 ? 4 : rows == 2 ? 2 : 1, part = warp % team;
+        // warps to a row: all four have the only token, two each of two, else every warp has up to four rows of its own, which
+        // it reads side by side
+        const int team = rows == 1 ? 4 : rows == 2 ? 2 : 1, part = warp % team, first_row = warp / team, pace = 4 / team;
+        // where a row is short its largest magnitude is found by every CTA, else its parts' are exchanged
+        const bool whole = split == 1 || args.whole_rows;
+        const long long c0 = whole ? 0 : (long long)k0 * 128, c1 = whole ? a.p.k : (long long)(k0 + nk) * 128;
         if (threadIdx.x < kTokenRows) part_most[threadIdx.x] = 0;
-        __syncthreads();
-        for (int r = warp / team; r < rows; r += 4 / team) {
-            uint32_t most = 0;
-            for (long long c = (long long)k0 * 128 + (part * 32 + lane) * 8; c < (long long)(k0 + nk) * 128; c += team * 256) {
-                Raw<X> raw;
-                load_raw(x + r * args.x_stride, c, a.p.k, args.x_vec, raw);
-                most_of(raw, most);
-            }
-            most = __reduce_max_sync(0xffffffffu, most_as_f32<X>(most));
-            if (lane == 0) atomicMax(&part_most[r], most);
+        uint32_t most[4] = {0, 0, 0, 0};
+        for (long long c = c0 + (part * 32 + lane) * 8; c < c1; c += team * 256) {
+            Raw<X> raw[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (first_row + i * pace < rows) load_raw(x + (first_row + i * pace) * args.x_stride, c, a.p.k, args.x_vec, raw[i]);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (first_row + i * pace < rows) most_of(raw[i], most[i]);
         }
-        if (split > 1) cluster_sync();
-        else __syncthreads();
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t all = __reduce_max_sync(0xffffffffu, most_as_f32<X>(most[i]));
+            if (lane == 0 && first_row + i * pace < rows) atomicMax(&part_most[first_row + i * pace], all);
+        }
+        if (whole) __syncthreads();
+        else cluster_sync();
         if (threadIdx.x < kTokenRows) {
-            uint32_t most = 0;
-            for (int r = 0; r < split; r++) {
-                uint32_t v = part_most[threadIdx.x];
-                if (split > 1)
+            uint32_t all = part_most[threadIdx.x];
+            if (!whole)
+                for (int r = 0; r < split; r++) {
+                    uint32_t v;
                     asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(map_rank(smem_addr(&part_most[threadIdx.x]), r)) : "memory");
-                most = max(most, v);
-            }
-            const bool fine = most < 0x7f800000u, live = fine && most != 0;
-            row_a[threadIdx.x] = live ? __uint_as_float(most) : 0.f;
-            row_inv[threadIdx.x] = live ? inverse_of(__uint_as_float(most)) : 0.f;
-            row_s[threadIdx.x] = fine ? __fdiv_rn(__uint_as_float(most), 127.f) : __uint_as_float(0x7fc00000u);
+                    all = max(all, v);
+                }
+            const bool fine = all < 0x7f800000u, live = fine && all != 0;
+            row_a[threadIdx.x] = live ? __uint_as_float(all) : 0.f;
+            row_inv[threadIdx.x] = live ? inverse_of(__uint_as_float(all)) : 0.f;
+            row_s[threadIdx.x] = fine ? __fdiv_rn(__uint_as_float(all), 127.f) : __uint_as_float(0x7fc00000u);
         }
+        __syncwarp();
+        take_tmem();
         __syncthreads();
-        for (int r = warp / team; r < rows; r += 4 / team) {
-            const float most = row_a[r], inv = row_inv[r];
-            for (int c = (part * 32 + lane) * 8; c < nk * 128; c += team * 256) {
-                Raw<X> raw;
+        for (int c = (part * 32 + lane) * 8; c < nk * 128; c += team * 256) {
+            Raw<X> raw[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (first_row + i * pace < rows)
+                    load_raw(x + (first_row + i * pace) * args.x_stride, (long long)k0 * 128 + c, a.p.k, args.x_vec, raw[i]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = first_row + i * pace;
+                if (r >= rows) continue;
                 float f[8];
-                load_raw(x + r * args.x_stride, (long long)k0 * 128 + c, a.p.k, args.x_vec, raw);
-                widen(raw, f);
-                const uint2 q = most > 0.f ? quant8<sizeof(X) == 2>(f, most, inv) : make_uint2(0u, 0u);
+                widen(raw[i], f);
+                const float largest = row_a[r];
+                const uint2 q = largest > 0.f ? quant8<sizeof(X) == 2>(f, largest, row_inv[r]) : make_uint2(0u, 0u);
                 asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(tokens0 + (c >> 7) * kTokenBlockBytes + r * 128 +
                                                                      ((((c >> 4) & 7) ^ (r & 7)) << 4) + (c & 8)),
                              "r"(q.x), "r"(q.y) : "memory");
@@ -533,12 +570,9 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
         }
         // what was written is visible to the tensor core's reads
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    // TMEM from here on: while a CTA holds some it waits for nobody but its own copies and products, so that whoever waits for
-    // TMEM on this SM (of whatever kernel) always gets it
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"((uint32_t)a.tmem_cols) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        __syncwarp();
+    } else {
+        take_tmem();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -584,7 +618,8 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
                         "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
                         "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
                         "l"(dw + q * adv_w), "l"(dx + q * adv_x), "r"(idesc), "r"((uint32_t)(i | q)) : "memory");
-                asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(empty(s)) : "memory");
+                if (i + a.stages < nk) // (filled again)
+                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(empty(s)) : "memory");
                 if (++s == a.stages) s = 0, phase ^= 1;
             }
             // (after a wait that gave up: of what was issued)
@@ -635,8 +670,11 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
         for (int i = 0; i < 16; i++)
             if (c + i < rows) red[(c + i) * 128 + warp * 32 + lane] = v[i];
     }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     free_tmem();
-    cluster_sync();
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     const long long col = col0 + lane * 4;
     const int live = a.p.n - col < 4 ? (int)(a.p.n - col) : 4;
     if (live > 0) {
@@ -767,11 +805,14 @@ long long split_shape(SplitProblem *a, const I8Product &p)
     return a->tiles_j * ((p.m + a->rows - 1) / a->rows);
 }
 
-// CTAs that share a contraction: as many as leave each a step of 128 and the GPU two CTAs an SM
+// CTAs that share a contraction: as many as leave each a step of 128 and all of them on the GPU at once.  One CTA that uses
+// TMEM fits an SM, and clusters of 1, 2, 4 and 8 leave some of the 148 SMs out (132 and 120 of them can be had by 4 and 8).
 int split_of(long long tiles, int k_blocks)
 {
+    const int most[4] = {148, 148, 132, 120};
     int split = 1;
-    while (split < 8 && split * 2 <= k_blocks && tiles * split * 2 <= 2 * 148) split *= 2;
+    for (int i = 1; i < 4 && (1 << i) <= k_blocks; i++)
+        if (tiles << i <= most[i]) split = 1 << i;
     return split;
 }
 
@@ -829,7 +870,8 @@ bool i8_tokens_fit(long long m, long long n, long long k, int kernel)
     if (m > kTokenRows || kernel == REXSC_INT8_PAIR) return false;
     const long long k_blocks = i8_tiles(k);
     const int split = split_of((n + 127) / 128, (int)k_blocks);
-    return (k_blocks + split - 1) / split <= kTokenMaxBlocks;
+    const long long steps = (k_blocks + split - 1) / split;
+    return steps <= kTokenMaxBlocks && m * steps * 128 <= kTokenMaxValues;
 }
 
 int launch_i8_tokens(const void *x, int dtype, long long stride, const I8Product &p, cudaStream_t st)
@@ -842,6 +884,8 @@ int launch_i8_tokens(const void *x, int dtype, long long stride, const I8Product
     a.first = (unsigned)(tiles * a.split);
     a.x = x;
     a.x_stride = stride;
+    // (16 KiB: a CTA's 128 threads read that much in about the time that an exchange within the cluster takes)
+    a.whole_rows = p.m * p.k * (long long)dtype_bytes(dtype) <= 16 * 1024;
     a.x_vec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(stride * (long long)dtype_bytes(dtype))) & 15) == 0;
     const auto kernel = dtype == REXSC_F32 ? product_split_kernel<float> : dtype == REXSC_F16 ? product_split_kernel<__half> : product_split_kernel<__nv_bfloat16>;
     return launch_cluster(kernel, a, tiles * a.split, a.split, kSplitThreads, smem, false, st, "product_split_kernel");

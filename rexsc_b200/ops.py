@@ -827,10 +827,10 @@ class _Int8Linear(torch.autograd.Function):
     def forward(ctx, x, weight, prepared, bias):
         dev = x.device
         n, k = (weight if prepared is None else prepared).shape
-        xt = x.dtype
-        x2 = _rows_of(x, k)
-        m = x2.shape[0]
-        ctx.lead = x.shape[:-1]
+        xt, lead = x.dtype, x.shape[:-1]
+        x2 = x if len(lead) == 1 and xt in _DTYPES and x.stride(1) == 1 else _rows_of(x, k)
+        m = x2.size(0)
+        ctx.lead = lead
         ctx.dtypes = xt, None if weight is None else weight.dtype, None if bias is None else bias.dtype
         ctx.sizes = m, n, k
         if m == 0:
@@ -845,7 +845,7 @@ class _Int8Linear(torch.autograd.Function):
             base = buf.data_ptr()
             xs = base + _tile_bytes(m, k)
             if prepared is None:
-                w2 = _rows_of(weight, k)
+                w2 = weight if weight.dtype in _DTYPES and weight.stride(1) == 1 else _rows_of(weight, k)
                 wd, w_ptr, w_dtype, w_stride = base + at_w, w2.data_ptr(), _DTYPES[w2.dtype], w2.stride(0)
                 ws = wd + _tile_bytes(n, k)
             else:
@@ -867,11 +867,15 @@ class _Int8Linear(torch.autograd.Function):
                 kept = (buf, None, None)
         ctx.save_for_backward(*kept)
         ctx.at_w = 0 if want_x and not want_w else at_w
-        return y if len(ctx.lead) == 1 else y.view(*ctx.lead, n)
+        return y if len(lead) == 1 else y.view(*lead, n)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        # (a graph of the backward pass is asked for: its nodes raise when they are used.  The wrapper costs the host 5 us)
+        return _int8_linear_once(ctx, dy) if torch.is_grad_enabled() else _Int8Linear.gradients(ctx, dy)
+
+    @staticmethod
+    def gradients(ctx, dy):
         m, n, k = ctx.sizes
         want_dx, want_dw, _, want_db = ctx.needs_input_grad
         xt, wt, bt = ctx.dtypes
@@ -889,27 +893,36 @@ class _Int8Linear(torch.autograd.Function):
                 ws = wd + _tile_bytes(n, k)
             if wdata is not None:
                 wd, ws = wdata.data_ptr(), wscale.data_ptr()
-            g = _rows_of(dy, n)
-            dx = torch.empty((m, k), dtype=xt if xt in _DTYPES else torch.float32, device=dev) if want_dx else None
-            dw = torch.empty((n, k), dtype=wt if wt in _DTYPES else torch.float32, device=dev) if want_dw else None
-            db = torch.empty((n,), dtype=bt if bt in _DTYPES else torch.float32, device=dev) if want_db else None
+            g = dy if dy.dim() == 2 and dy.dtype in _DTYPES and dy.stride(1) == 1 else _rows_of(dy, n)
+            dx = dw = db = None
+            dx_ptr = dw_ptr = db_ptr = dx_code = dw_code = db_code = 0
+            if want_dx:
+                dx = g.new_empty((m, k), dtype=xt if xt in _DTYPES else torch.float32)
+                dx_ptr, dx_code = dx.data_ptr(), _DTYPES[dx.dtype]
+            if want_dw:
+                dw = g.new_empty((n, k), dtype=wt if wt in _DTYPES else torch.float32)
+                dw_ptr, dw_code = dw.data_ptr(), _DTYPES[dw.dtype]
+            if want_db:
+                db = g.new_empty((n,), dtype=bt if bt in _DTYPES else torch.float32)
+                db_ptr, db_code = db.data_ptr(), _DTYPES[db.dtype]
             nbytes = _int8_bwd_scratch(m, n, want_dx, want_dw, want_db)
             scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            ptr = lambda t: 0 if t is None else t.data_ptr()
-            code = lambda t: 0 if t is None else _DTYPES[t.dtype]
-            rc = _lib.load().rexsc_int8_linear_bwd(g.data_ptr(), _DTYPES[g.dtype], m, n, k, g.stride(0), xd, xs, wd, ws,
-                                                   ptr(dx), code(dx), ptr(dw), code(dw), ptr(db), code(db), ctx.kernel,
-                                                   scratch.data_ptr(), nbytes, _stream(dev))
+            rc = _lib.load().rexsc_int8_linear_bwd(g.data_ptr(), _DTYPES[g.dtype], m, n, k, g.stride(0), xd, xs, wd, ws, dx_ptr,
+                                                   dx_code, dw_ptr, dw_code, db_ptr, db_code, ctx.kernel, scratch.data_ptr(),
+                                                   nbytes, _stream(dev))
             if rc:
                 _lib.check(rc, "rexsc_int8_linear_bwd")
-            if dx is not None:
+            if want_dx:
                 dx = dx if len(ctx.lead) == 1 else dx.view(*ctx.lead, k)
                 dx = dx if dx.dtype == xt else dx.to(xt)
-            if dw is not None and dw.dtype != wt:
+            if want_dw and dw.dtype != wt:
                 dw = dw.to(wt)
-            if db is not None and db.dtype != bt:
+            if want_db and db.dtype != bt:
                 db = db.to(bt)
             return dx, dw, None, db
+
+
+_int8_linear_once = torch.autograd.function.once_differentiable(_Int8Linear.gradients)
 
 
 @_traced

@@ -20,7 +20,8 @@ def test_sizes_of_8_bit_matrices(lib):
     for rows, cols in [(0, 1), (1, 0), (-1, 5), ((1 << 30) + 1, 1)]:
         assert lib.rexsc_int8_data_size(rows, cols) == 0
     assert lib.rexsc_int8_linear_workspace_size(17, 4096, 4096, 0) == 256 + 32 * tile
-    assert lib.rexsc_int8_linear_workspace_size(16, 4096, 4096, 0) == 0          # the product's kernel quantises a few tokens
+    assert lib.rexsc_int8_linear_workspace_size(2, 4096, 4096, 0) == 0           # the product's kernel quantises a few tokens
+    assert lib.rexsc_int8_linear_workspace_size(16, 512, 512, 0) == 0
     assert lib.rexsc_int8_linear_workspace_size(16, 4096, 4096, 2) == 256 + 32 * tile
     assert lib.rexsc_int8_linear_workspace_size(1, 8, 131071, 0) == 256 + 1024 * tile   # too long for that
     assert lib.rexsc_int8_linear_workspace_size(17, 4096, 131072, 0) == 0
