@@ -10,9 +10,10 @@
 //   product_split_kernel 128 columns of the output (lanes of TMEM) x 16 to 128 rows per CTA; the CTAs of a cluster split the
 //                        contraction and join their int32 sums through distributed shared memory (whole numbers: the
 //                        order does not matter).  It takes two products in one launch (a layer's two gradients), and up
-//                        to 16 tokens as they are, which it quantises itself.
+//                        to 32 tokens as they are, which it quantises itself.
 // Every mbarrier wait is bounded; a CTA whose wait gives up raises the library's status word (rexsc_int8_status), stores
 // nothing more, waits for its copies in flight, frees its TMEM and leaves.
+#include <atomic>
 #include <cuda.h>
 
 #include "int8_quant.cuh"
@@ -44,6 +45,11 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity)
     }
     atomicExch(&g_i8_status, 1);
     return false;
+}
+// by a whole warp, with one answer
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes)
 {
@@ -100,6 +106,40 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t saddr)
     d |= (uint64_t)2 << 61;
     return d;
 }
+// Four products (128 of the contraction) and a commit, by a converged warp of which one lane issues them: kept out of a
+// one-lane branch, the descriptors stay in uniform registers.  (From such a branch a step took 472 cycles to issue whatever
+// its size, 512 x 4096 x 4096 on the split kernel 33 us.)
+template <int kCtas>
+__device__ __forceinline__ void product_step(uint32_t tmem, uint64_t da, uint64_t db, uint32_t adv_a, uint32_t adv_b,
+                                             uint32_t idesc, bool add)
+{
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        if (kCtas == 2)
+            asm volatile(
+                "{\n\t.reg .pred p, e;\n\tsetp.ne.u32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+                "@e tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+                "l"(da + q * adv_a), "l"(db + q * adv_b), "r"(idesc), "r"((uint32_t)(add || q)) : "memory");
+        else
+            asm volatile(
+                "{\n\t.reg .pred p, e;\n\tsetp.ne.u32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+                "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
+                "l"(da + q * adv_a), "l"(db + q * adv_b), "r"(idesc), "r"((uint32_t)(add || q)) : "memory");
+    }
+}
+__device__ __forceinline__ void commit_one(uint32_t bar)
+{
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t bar, uint32_t ctas)
+{
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+                 "h"((uint16_t)ctas) : "memory");
+}
+// the warp's number as a value that is the same for all of it
+__device__ __forceinline__ int warp_number() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
 // instruction descriptor: int32 sums, signed 8-bit operands, their major-ness, M and N
 __host__ __device__ __forceinline__ uint32_t product_idesc(int m, int n, int a_mn, int b_mn)
 {
@@ -230,7 +270,7 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
     auto acc_empty = [&](int b) { return bar0 + (2 * kPairStages + 2 + b) * 8; };
     const uint32_t drained = bar0 + (2 * kPairStages + 4) * 8;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_number(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const long long first = blockIdx.x >> 1, step = gridDim.x >> 1, tiles = a.tiles_i * a.tiles_j;
 
@@ -298,7 +338,7 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) { // ---- products
+        if (rank == 0) { // ---- products
             const uint32_t idesc = product_idesc(256, 256, a.p.a.mn_major, a.p.b.mn_major);
             const uint32_t adv_a = a.p.a.mn_major ? 4096 >> 4 : 32 >> 4, adv_b = a.p.b.mn_major ? 4096 >> 4 : 32 >> 4;
             const uint64_t desc0 = tile_desc(smem_addr(smem));
@@ -307,31 +347,21 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
             bool ok = true;
             for (long long t = first; t < tiles && ok; t += step, turn++) {
                 const int b = turn & 1;
-                if (turn >= 2 && !(ok = mbar_wait(acc_empty(b), (turn / 2 - 1) & 1))) break;
+                if (turn >= 2 && !(ok = mbar_wait_warp(acc_empty(b), (turn / 2 - 1) & 1))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (int k = 0; k < a.k_blocks; k++) {
-                    if (!(ok = mbar_wait(full(r.at), r.phase))) break;
+                    if (!(ok = mbar_wait_warp(full(r.at), r.phase))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t da = desc0 + r.at * (kPairStageBytes >> 4), db = da + (kI8TileBytes >> 4);
-#pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        asm volatile(
-                            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + b * 256),
-                            "l"(da + q * adv_a), "l"(db + q * adv_b), "r"(idesc), "r"((uint32_t)(k | q)) : "memory");
-                    asm volatile(
-                        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                            empty(r.at)), "h"((uint16_t)3) : "memory");
+                    const uint64_t da = desc0 + r.at * (kPairStageBytes >> 4);
+                    product_step<2>(tmem + b * 256, da, da + (kI8TileBytes >> 4), adv_a, adv_b, idesc, k > 0);
+                    commit_pair(empty(r.at), 3);
                     r.next();
                 }
-                if (ok)
-                    asm volatile(
-                        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                            acc_full(b)), "h"((uint16_t)3) : "memory");
+                if (ok) commit_pair(acc_full(b), 3);
             }
             if (!ok) { // products in flight read both CTAs' stages and write their accumulators
-                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drained) : "memory");
-                mbar_wait(drained, 0);
+                commit_pair(drained, 1);
+                mbar_wait_warp(drained, 0);
             }
         }
     } else { // ---- epilogue: a lane per row of this CTA's 128
@@ -423,10 +453,8 @@ struct SplitArgs {
 constexpr int kSplitThreads = 128;
 constexpr int kSplitMaxStages = 12;
 constexpr size_t kSplitSmemMost = 212 * 1024;
-constexpr int kTokenRows = 16;                      // most tokens that the kernel quantises by itself
-constexpr int kTokenBlockBytes = kTokenRows * 128;  // 128 columns of them
-constexpr int kTokenMaxBlocks = 32;                 // such blocks a CTA holds
-constexpr int kTokenMaxValues = 8192;               // values a CTA quantises at the most: with more of them a launch of its own
+constexpr int kTokenRows = 32;                      // most tokens that the kernel quantises by itself
+constexpr int kTokenMaxValues = 4096;               // values a CTA quantises at the most: with more of them a launch of its own
                                                     // is sooner done (13 x 2051 fp16 on 5003 channels: 23 us here, 9 us so)
 
 __device__ __forceinline__ void store1(void *out, int dtype, long long i, float v)
@@ -453,7 +481,7 @@ __device__ __forceinline__ void store4(void *out, int dtype, long long i, const 
     }
 }
 
-// X: int8_t where the rows operand is a matrix of tiles; else the type of up to 16 tokens that every CTA quantises for itself,
+// X: int8_t where the rows operand is a matrix of tiles; else the type of up to 32 tokens that every CTA quantises for itself,
 // its part of the contraction only: the CTAs of a cluster tell one another the largest magnitudes of their parts.
 template <typename X>
 __global__ void __launch_bounds__(kSplitThreads)
@@ -470,7 +498,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
     auto full = [&](int s) { return bar0 + s * 8; };
     auto empty = [&](int s) { return bar0 + (kSplitMaxStages + s) * 8; };
     const uint32_t acc_full = bar0 + 2 * kSplitMaxStages * 8;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = warp_number(), lane = threadIdx.x & 31;
     const int which = !kTokens && blockIdx.x >= args.first;
     const SplitProblem &a = args.p[which];
     const int split = args.split, rank = split > 1 ? (int)cluster_rank() : 0;
@@ -480,7 +508,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
     const long long row0 = ti * a.rows, col0 = tj * 128;
     const int rows = a.p.m - row0 < a.rows ? (int)(a.p.m - row0) : a.rows; // that exist
     const uint32_t smem0 = smem_addr(smem), stage_bytes = kI8TileBytes + (kTokens ? 0 : a.q_bytes);
-    const uint32_t tokens0 = smem0 + a.stages * stage_bytes; // the quantised tokens, [128 columns][16][128 bytes]
+    const uint32_t tokens0 = smem0 + a.stages * stage_bytes; // the quantised tokens, [128 columns][rows][128 bytes]
     const int early = nk < a.stages ? nk : a.stages;
 
     const int8_t *pw = a.p.b.data + ((size_t)(tj * a.p.b.step_mn) + (size_t)(k0 * a.p.b.step_k)) * kI8TileBytes;
@@ -508,28 +536,31 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
     __syncwarp();
     if constexpr (kTokens) {
         const X *x = static_cast<const X *>(args.x);
-        // warps to a row: all four have the only token, two each of two, else every warp has up to four rows of its own, which
+        // warps to a row: all four have the only token, two each of two, else every warp has rows of its own, four of which
         // it reads side by side
         const int team = rows == 1 ? 4 : rows == 2 ? 2 : 1, part = warp % team, first_row = warp / team, pace = 4 / team;
         // where a row is short its largest magnitude is found by every CTA, else its parts' are exchanged
         const bool whole = split == 1 || args.whole_rows;
         const long long c0 = whole ? 0 : (long long)k0 * 128, c1 = whole ? a.p.k : (long long)(k0 + nk) * 128;
         if (threadIdx.x < kTokenRows) part_most[threadIdx.x] = 0;
-        uint32_t most[4] = {0, 0, 0, 0};
-        for (long long c = c0 + (part * 32 + lane) * 8; c < c1; c += team * 256) {
-            Raw<X> raw[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (first_row + i * pace < rows) load_raw(x + (first_row + i * pace) * args.x_stride, c, a.p.k, args.x_vec, raw[i]);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (first_row + i * pace < rows) most_of(raw[i], most[i]);
-        }
         __syncthreads();
+        for (int r0 = first_row; r0 < rows; r0 += 4 * pace) {
+            uint32_t most[4] = {0, 0, 0, 0};
+            for (long long c = c0 + (part * 32 + lane) * 8; c < c1; c += team * 256) {
+                Raw<X> raw[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t all = __reduce_max_sync(0xffffffffu, most_as_f32<X>(most[i]));
-            if (lane == 0 && first_row + i * pace < rows) atomicMax(&part_most[first_row + i * pace], all);
+                for (int i = 0; i < 4; i++)
+                    if (r0 + i * pace < rows) load_raw(x + (r0 + i * pace) * args.x_stride, c, a.p.k, args.x_vec, raw[i]);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (r0 + i * pace < rows) most_of(raw[i], most[i]);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t all = __reduce_max_sync(0xffffffffu, most_as_f32<X>(most[i]));
+                if (lane == 0 && r0 + i * pace < rows) atomicMax(&part_most[r0 + i * pace], all);
+            }
         }
         if (whole) __syncthreads();
         else cluster_sync();
@@ -549,25 +580,26 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
         __syncwarp();
         take_tmem();
         __syncthreads();
-        for (int c = (part * 32 + lane) * 8; c < nk * 128; c += team * 256) {
-            Raw<X> raw[4];
+        for (int r0 = first_row; r0 < rows; r0 += 4 * pace)
+            for (int c = (part * 32 + lane) * 8; c < nk * 128; c += team * 256) {
+                Raw<X> raw[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (first_row + i * pace < rows)
-                    load_raw(x + (first_row + i * pace) * args.x_stride, (long long)k0 * 128 + c, a.p.k, args.x_vec, raw[i]);
+                for (int i = 0; i < 4; i++)
+                    if (r0 + i * pace < rows)
+                        load_raw(x + (r0 + i * pace) * args.x_stride, (long long)k0 * 128 + c, a.p.k, args.x_vec, raw[i]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int r = first_row + i * pace;
-                if (r >= rows) continue;
-                float f[8];
-                widen(raw[i], f);
-                const float largest = row_a[r];
-                const uint2 q = largest > 0.f ? quant8<sizeof(X) == 2>(f, largest, row_inv[r]) : make_uint2(0u, 0u);
-                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(tokens0 + (c >> 7) * kTokenBlockBytes + r * 128 +
-                                                                     ((((c >> 4) & 7) ^ (r & 7)) << 4) + (c & 8)),
-                             "r"(q.x), "r"(q.y) : "memory");
+                for (int i = 0; i < 4; i++) {
+                    const int r = r0 + i * pace;
+                    if (r >= rows) continue;
+                    float f[8];
+                    widen(raw[i], f);
+                    const float largest = row_a[r];
+                    const uint2 q = largest > 0.f ? quant8<sizeof(X) == 2>(f, largest, row_inv[r]) : make_uint2(0u, 0u);
+                    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(tokens0 + (c >> 7) * a.q_bytes + r * 128 +
+                                                                         ((((c >> 4) & 7) ^ (r & 7)) << 4) + (c & 8)),
+                                 "r"(q.x), "r"(q.y) : "memory");
+                }
             }
-        }
         // what was written is visible to the tensor core's reads
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -603,28 +635,20 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
             for (int j = filled < a.stages ? 0 : filled - a.stages; j < filled; j++) mbar_wait(full(j % a.stages), (j / a.stages) & 1);
         }
     } else if (warp == 1) {
-        if (lane == 0) { // ---- products: lanes are output columns, columns of TMEM output rows
-            const uint32_t idesc = product_idesc(128, a.rows, a.p.b.mn_major, a.p.a.mn_major);
-            const uint32_t adv_w = a.p.b.mn_major ? 4096 >> 4 : 32 >> 4, adv_x = a.p.a.mn_major ? 4096 >> 4 : 32 >> 4;
-            int s = 0, phase = 0;
-            for (int i = 0; i < nk; i++) {
-                if (!mbar_wait(full(s), phase)) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t sa = smem0 + s * stage_bytes;
-                const uint64_t dw = tile_desc(sa), dx = tile_desc(kTokens ? tokens0 + i * kTokenBlockBytes : sa + kI8TileBytes);
-#pragma unroll
-                for (int q = 0; q < 4; q++)
-                    asm volatile(
-                        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem),
-                        "l"(dw + q * adv_w), "l"(dx + q * adv_x), "r"(idesc), "r"((uint32_t)(i | q)) : "memory");
-                if (i + a.stages < nk) // (filled again)
-                    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(empty(s)) : "memory");
-                if (++s == a.stages) s = 0, phase ^= 1;
-            }
-            // (after a wait that gave up: of what was issued)
-            asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(acc_full) : "memory");
+        // ---- products: lanes are output columns, columns of TMEM output rows
+        const uint32_t idesc = product_idesc(128, a.rows, a.p.b.mn_major, a.p.a.mn_major);
+        const uint32_t adv_w = a.p.b.mn_major ? 4096 >> 4 : 32 >> 4, adv_x = a.p.a.mn_major ? 4096 >> 4 : 32 >> 4;
+        const uint64_t desc_w = tile_desc(smem0), desc_x = tile_desc(kTokens ? tokens0 : smem0 + kI8TileBytes);
+        int s = 0, phase = 0;
+        for (int i = 0; i < nk; i++) {
+            if (!mbar_wait_warp(full(s), phase)) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            product_step<1>(tmem, desc_w + (s * stage_bytes >> 4), desc_x + ((kTokens ? i * a.q_bytes : s * stage_bytes) >> 4),
+                            adv_w, adv_x, idesc, i > 0);
+            if (i + a.stages < nk) commit_one(empty(s)); // (filled again)
+            if (++s == a.stages) s = 0, phase ^= 1;
         }
+        commit_one(acc_full); // (after a wait that gave up: of what was issued)
     }
     __syncwarp();
     if (!kTokens) wait_previous_launch();
@@ -710,12 +734,21 @@ int store_alignment(const I8Product &p)
     return bits & 15 ? 0 : bits & 31 ? 16 : 32;
 }
 
-template <typename Args>
-int launch_cluster(void (*kernel)(Args), const Args &args, long long blocks, int cluster, int threads, size_t smem, bool overlap,
-                   cudaStream_t st, const char *name)
+// kSmemMost: what any launch of the kernel asks for.  The kernel is allowed that much once per device (and not what a launch
+// needs: two threads would take it from one another).
+template <auto kKernel, size_t kSmemMost, typename Args>
+int launch_cluster(const Args &args, long long blocks, int cluster, int threads, size_t smem, bool overlap, cudaStream_t st,
+                   const char *name)
 {
     if (blocks > 0x7fffffffll) return REXSC_E_UNSUPPORTED;
-    REXSC_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static std::atomic<unsigned long long> allowed{0};
+    int device = 0;
+    REXSC_CUDA_CHECK(cudaGetDevice(&device));
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+        REXSC_CUDA_CHECK(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost));
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3((unsigned)threads);
@@ -736,7 +769,7 @@ int launch_cluster(void (*kernel)(Args), const Args &args, long long blocks, int
     }
     cfg.attrs = attr;
     cfg.numAttrs = (unsigned)n;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kKernel, args);
     note_kernel_launch();
     if (e != cudaSuccess) {
         cudaGetLastError();
@@ -783,7 +816,7 @@ int launch_pair(const I8Product &p, bool overlap, cudaStream_t st)
     a.k_blocks = (int)i8_tiles(p.k);
     a.store_bytes = store_alignment(p);
     const long long tiles = a.tiles_i * a.tiles_j, pairs = tiles < 74 ? tiles : 74;
-    return launch_cluster(product_pair_kernel<T>, a, pairs * 2, 0, kPairThreads, kPairSmem, overlap, st, "product_pair_kernel");
+    return launch_cluster<product_pair_kernel<T>, kPairSmem>(a, pairs * 2, 0, kPairThreads, kPairSmem, overlap, st, "product_pair_kernel");
 }
 
 // ---- which kernel, and its shape
@@ -819,7 +852,7 @@ int split_of(long long tiles, int k_blocks)
 // stages of a CTA, and the shared memory that it needs
 size_t split_stages(SplitProblem *a, int split, bool tokens)
 {
-    const int steps = (a->k_blocks + split - 1) / split, fixed = tokens ? steps * kTokenBlockBytes : 0;
+    const int steps = (a->k_blocks + split - 1) / split, fixed = tokens ? steps * a->q_bytes : 0;
     const int stage = kI8TileBytes + (tokens ? 0 : a->q_bytes), most = ((int)kSplitSmemMost - 1024 - fixed) / stage;
     a->stages = steps < kSplitMaxStages ? steps : kSplitMaxStages;
     if (a->stages > most) a->stages = most;
@@ -842,8 +875,8 @@ int launch_split(const I8Product &p, const I8Product *second, bool overlap, cuda
     }
     if ((tiles + more) * a.split > 0x7fffffffll) return REXSC_E_UNSUPPORTED;
     a.first = (unsigned)(tiles * a.split);
-    return launch_cluster(product_split_kernel<int8_t>, a, (tiles + more) * a.split, a.split, kSplitThreads, smem, overlap, st,
-                          "product_split_kernel");
+    return launch_cluster<product_split_kernel<int8_t>, kSplitSmemMost>(a, (tiles + more) * a.split, a.split, kSplitThreads, smem,
+                                                                        overlap, st, "product_split_kernel");
 }
 
 } // namespace
@@ -870,8 +903,7 @@ bool i8_tokens_fit(long long m, long long n, long long k, int kernel)
     if (m > kTokenRows || kernel == REXSC_INT8_PAIR) return false;
     const long long k_blocks = i8_tiles(k);
     const int split = split_of((n + 127) / 128, (int)k_blocks);
-    const long long steps = (k_blocks + split - 1) / split;
-    return steps <= kTokenMaxBlocks && m * steps * 128 <= kTokenMaxValues;
+    return m * ((k_blocks + split - 1) / split) * 128 <= kTokenMaxValues;
 }
 
 int launch_i8_tokens(const void *x, int dtype, long long stride, const I8Product &p, cudaStream_t st)
@@ -887,8 +919,11 @@ int launch_i8_tokens(const void *x, int dtype, long long stride, const I8Product
     // (16 KiB: a CTA's 128 threads read that much in about the time that an exchange within the cluster takes)
     a.whole_rows = p.m * p.k * (long long)dtype_bytes(dtype) <= 16 * 1024;
     a.x_vec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(stride * (long long)dtype_bytes(dtype))) & 15) == 0;
-    const auto kernel = dtype == REXSC_F32 ? product_split_kernel<float> : dtype == REXSC_F16 ? product_split_kernel<__half> : product_split_kernel<__nv_bfloat16>;
-    return launch_cluster(kernel, a, tiles * a.split, a.split, kSplitThreads, smem, false, st, "product_split_kernel");
+#define REXSC_I8_TOKENS(X)                                                                                             \
+    launch_cluster<product_split_kernel<X>, kSplitSmemMost>(a, tiles *a.split, a.split, kSplitThreads, smem, false, st, \
+                                                            "product_split_kernel")
+    return dtype == REXSC_F32 ? REXSC_I8_TOKENS(float) : dtype == REXSC_F16 ? REXSC_I8_TOKENS(__half) : REXSC_I8_TOKENS(__nv_bfloat16);
+#undef REXSC_I8_TOKENS
 }
 
 } // namespace rexsc

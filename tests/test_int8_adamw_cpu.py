@@ -20,7 +20,7 @@ def test_sizes_of_8_bit_matrices(lib):
     for rows, cols in [(0, 1), (1, 0), (-1, 5), ((1 << 30) + 1, 1)]:
         assert lib.rexsc_int8_data_size(rows, cols) == 0
     assert lib.rexsc_int8_linear_workspace_size(17, 4096, 4096, 0) == 256 + 32 * tile
-    assert lib.rexsc_int8_linear_workspace_size(2, 4096, 4096, 0) == 0           # the product's kernel quantises a few tokens
+    assert lib.rexsc_int8_linear_workspace_size(4, 4096, 4096, 0) == 0           # the product's kernel quantises a few tokens
     assert lib.rexsc_int8_linear_workspace_size(16, 512, 512, 0) == 0
     assert lib.rexsc_int8_linear_workspace_size(16, 4096, 4096, 2) == 256 + 32 * tile
     assert lib.rexsc_int8_linear_workspace_size(1, 8, 131071, 0) == 256 + 1024 * tile   # too long for that
@@ -49,9 +49,9 @@ def test_int8_entry_points_refuse_bad_arguments(lib):
     assert mm(p, None, p, p, None, 0, 4, 4, 128, p, 0, 0, None) == -1
     assert mm(off, p, p, p, None, 0, 4, 4, 128, p, 0, 0, None) == -1
     fwd = lib.rexsc_int8_linear_fwd
-    assert fwd(p, 0, 40, 128, 128, p, p, 8, None, 0, p, 0, 0, None, 0, None) == -3
-    assert fwd(p, 0, 40, 128, 128, p, p, 8, None, 0, p, 0, 0, p, 256, None) == -3
-    assert fwd(p, 0, 40, 128, 128, off, p, 8, None, 0, p, 0, 0, p, 1 << 30, None) == -1
+    assert fwd(p, 0, 400, 128, 128, p, p, 8, None, 0, p, 0, 0, None, 0, None) == -3
+    assert fwd(p, 0, 400, 128, 128, p, p, 8, None, 0, p, 0, 0, p, 256, None) == -3
+    assert fwd(p, 0, 400, 128, 128, off, p, 8, None, 0, p, 0, 0, p, 1 << 30, None) == -1
     train = lib.rexsc_int8_linear_train_fwd
     assert train(p, 0, 4, 128, 128, p, 0, 8, 128, None, 0, off, p, p, p, p, 0, 0, None) == -1
     assert train(p, 0, 4, 128, 128, p, 7, 8, 128, None, 0, p, p, p, p, p, 0, 0, None) == -1
