@@ -66,9 +66,16 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mapped)
 {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mapped) : "memory");
 }
-__device__ __forceinline__ void copy_in(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+// (these by one lane of a converged warp, for the reason that product_step has)
+__device__ __forceinline__ void mbar_expect_one(uint32_t bar, uint32_t bytes)
 {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_in_one(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}" ::"r"(dst),
                  "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 // A tile of a matrix of tiles (rows of 128 bytes) into this CTA's shared memory, its bytes counted by a barrier of either CTA of
@@ -492,7 +499,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
     __shared__ __align__(8) uint64_t bars[2 * kSplitMaxStages + 1];
     __shared__ uint32_t tmem_slot;
     __shared__ uint32_t part_most[kTokenRows];
-    __shared__ float row_a[kTokenRows], row_inv[kTokenRows], row_s[kTokenRows];
+    __shared__ float row_a[kTokenRows], row_inv[kTokenRows], row_s[kSplitThreads];
     uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     const uint32_t bar0 = smem_addr(bars);
     auto full = [&](int s) { return bar0 + s * 8; };
@@ -513,14 +520,17 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
 
     const int8_t *pw = a.p.b.data + ((size_t)(tj * a.p.b.step_mn) + (size_t)(k0 * a.p.b.step_k)) * kI8TileBytes;
     const size_t step_w = (size_t)a.p.b.step_k * kI8TileBytes;
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < a.stages; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
-        mbar_init(acc_full, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (warp == 0) {
+        if (lane == 0) {
+            for (int s = 0; s < a.stages; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+            mbar_init(acc_full, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
         // the weights depend neither on the tokens nor on the launch before, which quantises the rows: begin with them
         for (int s = 0; s < early; s++) {
-            mbar_expect(full(s), stage_bytes);
-            copy_in(smem0 + s * stage_bytes, pw, kI8TileBytes, full(s));
+            mbar_expect_one(full(s), stage_bytes);
+            copy_in_one(smem0 + s * stage_bytes, pw, kI8TileBytes, full(s));
             pw += step_w;
         }
     }
@@ -612,28 +622,27 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
     const uint32_t tmem = tmem_slot;
 
     if (warp == 0) {
-        if (lane == 0) { // ---- copies
-            const int8_t *px = a.p.a.data + ((size_t)((row0 >> 7) * a.p.a.step_mn) + (size_t)(k0 * a.p.a.step_k)) * kI8TileBytes +
-                               (a.p.a.mn_major ? 0 : (row0 & 127) * 128);
-            const size_t step_x = (size_t)a.p.a.step_k * kI8TileBytes;
-            auto copy_x = [&](int s) {
-                if (!kTokens) copy_in(smem0 + s * stage_bytes + kI8TileBytes, px, a.q_bytes, full(s));
-                px += step_x;
-            };
-            if (!kTokens) wait_previous_launch();
-            for (int s = 0; s < early; s++) copy_x(s);
-            int s = 0, phase = 0, filled = early;
-            for (; filled < nk; filled++) {
-                if (!mbar_wait(empty(s), phase)) break;
-                mbar_expect(full(s), stage_bytes);
-                copy_in(smem0 + s * stage_bytes, pw, kI8TileBytes, full(s));
-                pw += step_w;
-                copy_x(s);
-                if (++s == a.stages) s = 0, phase ^= 1;
-            }
-            // nothing on its way when this CTA leaves: the last filling of every stage
-            for (int j = filled < a.stages ? 0 : filled - a.stages; j < filled; j++) mbar_wait(full(j % a.stages), (j / a.stages) & 1);
+        // ---- copies
+        const int8_t *px = a.p.a.data + ((size_t)((row0 >> 7) * a.p.a.step_mn) + (size_t)(k0 * a.p.a.step_k)) * kI8TileBytes +
+                           (a.p.a.mn_major ? 0 : (row0 & 127) * 128);
+        const size_t step_x = (size_t)a.p.a.step_k * kI8TileBytes;
+        auto copy_x = [&](int s) {
+            if (!kTokens) copy_in_one(smem0 + s * stage_bytes + kI8TileBytes, px, a.q_bytes, full(s));
+            px += step_x;
+        };
+        if (!kTokens) wait_previous_launch();
+        for (int s = 0; s < early; s++) copy_x(s);
+        int s = 0, phase = 0, filled = early;
+        for (; filled < nk; filled++) {
+            if (!mbar_wait_warp(empty(s), phase)) break;
+            mbar_expect_one(full(s), stage_bytes);
+            copy_in_one(smem0 + s * stage_bytes, pw, kI8TileBytes, full(s));
+            pw += step_w;
+            copy_x(s);
+            if (++s == a.stages) s = 0, phase ^= 1;
         }
+        // nothing on its way when this CTA leaves: the last filling of every stage
+        for (int j = filled < a.stages ? 0 : filled - a.stages; j < filled; j++) mbar_wait_warp(full(j % a.stages), (j / a.stages) & 1);
     } else if (warp == 1) {
         // ---- products: lanes are output columns, columns of TMEM output rows
         const uint32_t idesc = product_idesc(128, a.rows, a.p.b.mn_major, a.p.a.mn_major);
@@ -651,7 +660,11 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
         commit_one(acc_full); // (after a wait that gave up: of what was issued)
     }
     __syncwarp();
-    if (!kTokens) wait_previous_launch();
+    if (!kTokens) {
+        wait_previous_launch();
+        if (threadIdx.x < rows) row_s[threadIdx.x] = a.p.row_scale[row0 + threadIdx.x];
+        __syncwarp();
+    }
     if (lane == 0) mbar_wait(acc_full, 0); // (one lane of a warp asks)
     __syncwarp();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -664,41 +677,21 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)a.tmem_cols) : "memory");
         }
     };
-    auto scale_of = [&](int r) { return kTokens ? row_s[r] : a.p.row_scale[row0 + r]; };
-    if (split == 1) {
-        const long long col = col0 + warp * 32 + lane;
-        const bool live = col < a.p.n;
-        const float cs = live && a.p.col_scale ? a.p.col_scale[col] : 1.f;
-        const float bias = live && a.p.bias ? load_any(a.p.bias, a.p.bias_dtype, col) : 0.f;
-        for (int c = 0; c < rows; c += 16) {
-            int v[16];
-            __syncwarp();
-            tmem_load16(tmem_lane + c, v);
-            if (live) {
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    if (c + i < rows)
-                        store1(a.p.out, a.p.out_dtype, (row0 + c + i) * a.p.out_stride + col, scaled(v[i], scale_of(c + i), cs, bias));
-            }
-        }
-        __syncwarp();
-        free_tmem();
-        return;
-    }
-    // sums to shared memory, [row][column]; every CTA of the cluster finishes some of the rows
+    // sums to shared memory, [row][column]; every CTA of the cluster finishes some of the rows, four columns a lane
     int *red = reinterpret_cast<int *>(smem);
     for (int c = 0; c < rows; c += 16) {
         int v[16];
+        __syncwarp();
         tmem_load16(tmem_lane + c, v);
 #pragma unroll
         for (int i = 0; i < 16; i++)
             if (c + i < rows) red[(c + i) * 128 + warp * 32 + lane] = v[i];
     }
     __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    free_tmem();
+    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    free_tmem(); // (its barrier is enough for a CTA alone)
     __syncwarp();
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     const long long col = col0 + lane * 4;
     const int live = a.p.n - col < 4 ? (int)(a.p.n - col) : 4;
     if (live > 0) {
@@ -709,22 +702,22 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
             bias[i] = i < live && a.p.bias ? load_any(a.p.bias, a.p.bias_dtype, col + i) : 0.f;
         }
         for (int c = rank * 4 + warp; c < rows; c += 4 * split) {
-            int4 sum = make_int4(0, 0, 0, 0);
+            int4 sum = *reinterpret_cast<const int4 *>(red + c * 128 + lane * 4);
             const uint32_t at = smem_addr(red + c * 128 + lane * 4);
-            for (int r = 0; r < split; r++) {
+            for (int i = 1; i < split; i++) {
+                const int r = (rank + i) & (split - 1); // (each starts with another one)
                 int4 v;
                 asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(map_rank(at, r)) : "memory");
                 sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
             }
-            const float rs = scale_of(c);
+            const float rs = row_s[c];
             const float f[4] = {scaled(sum.x, rs, cs[0], bias[0]), scaled(sum.y, rs, cs[1], bias[1]),
                                 scaled(sum.z, rs, cs[2], bias[2]), scaled(sum.w, rs, cs[3], bias[3])};
             store4(a.p.out, a.p.out_dtype, (row0 + c) * a.p.out_stride + col, f, live, a.store_bytes >= 16);
         }
     }
-    __syncwarp();
-    cluster_sync(); // the others still read this CTA's sums
+    if (split > 1) cluster_sync(); // the others still read this CTA's sums
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------
@@ -820,12 +813,6 @@ int launch_pair(const I8Product &p, bool overlap, cudaStream_t st)
 }
 
 // ---- which kernel, and its shape
-bool use_pairs(const I8Product &p, int kernel)
-{
-    const long long tiles = ((p.m + 255) / 256) * ((p.n + 255) / 256);
-    return kernel == REXSC_INT8_PAIR || (kernel == REXSC_INT8_AUTO && p.m > 128 && tiles >= 37);
-}
-
 long long split_shape(SplitProblem *a, const I8Product &p)
 {
     a->p = p;
@@ -849,6 +836,20 @@ int split_of(long long tiles, int k_blocks)
     return split;
 }
 
+// The kernel that takes less time by what they were measured at (us, B200, bf16): pairs 5.6 + 0.28 for every step of 128 along
+// the contraction and round of 74 output tiles; the split 2 and for every round of 148 CTAs 3 + 0.027 rows and for every step
+// of a CTA 0.14 + 0.0006 rows.  Whole calls: 1024 x 2048 x 512 pairs 9.9, split 12.3; 512 x 4096 x 4096 18.4 and 18.7;
+// 192 x 8192 x 8192 29.7 and 25.3; 64 x 8192 x 8192 26.0 and 15.6.
+bool use_pairs(const I8Product &p, int kernel)
+{
+    if (kernel != REXSC_INT8_AUTO) return kernel == REXSC_INT8_PAIR;
+    SplitProblem a;
+    const long long tiles = split_shape(&a, p), pairs = ((p.m + 255) / 256) * ((p.n + 255) / 256);
+    const int split = split_of(tiles, a.k_blocks);
+    const double rounds = (double)((tiles * split + 147) / 148), steps = (a.k_blocks + split - 1) / split;
+    return 5.6 + (double)((pairs + 73) / 74) * a.k_blocks * 0.28 < 2 + rounds * (3 + 0.027 * a.rows + steps * (0.14 + 0.0006 * a.rows));
+}
+
 // stages of a CTA, and the shared memory that it needs
 size_t split_stages(SplitProblem *a, int split, bool tokens)
 {
@@ -857,7 +858,7 @@ size_t split_stages(SplitProblem *a, int split, bool tokens)
     a->stages = steps < kSplitMaxStages ? steps : kSplitMaxStages;
     if (a->stages > most) a->stages = most;
     size_t smem = (size_t)a->stages * stage + fixed;
-    if (split > 1 && smem < (size_t)a->rows * 512) smem = (size_t)a->rows * 512;
+    if (smem < (size_t)a->rows * 512) smem = (size_t)a->rows * 512; // the sums
     return smem + 1024;
 }
 
