@@ -23,7 +23,7 @@ from typing import Dict, List, Optional
 import torch
 import torch.distributed as dist
 
-from .. import sharding
+from .. import optim, sharding
 
 IMAGENET_MEAN = (0.485, 0.456, 0.406)   # normalisation constants of main_imagenet.py:139-140
 IMAGENET_STD = (0.229, 0.224, 0.225)
@@ -43,7 +43,7 @@ class Workload:
     channels_last: bool
     generator: str = "lfsr"
     inputs: str = "imagenet"         # imagenet: clip(N(0,1),-3,3) normalised; cifar: U[0,1)
-    optimizer: str = "sgd"
+    optimizer: str = "sgd"           # sgd | adam | adamw | adamw8 (8-bit moments)
     acc_limit: int = 128             # samples accumulated before an optimizer step (the reference's default)
     extra: Dict = field(default_factory=dict)
 
@@ -142,9 +142,14 @@ class TimedLoader:
 
 
 def make_optimizer(wl: Workload, model, lr: float = 1e-3):
-    """SGD with the momentum of main_conv.py:232-233 (what the metric names), or Adam as main_imagenet.py:212-213."""
+    """SGD with the momentum of main_conv.py:232-233 (what the metric names), Adam as main_imagenet.py:212-213, or this
+    library's AdamW (:class:`rexsc_b200.optim.AdamW`, CUDA only) with moments in 32 or in 8 bits."""
     if wl.optimizer == "adam":
         return torch.optim.Adam(model.parameters(), lr=lr, weight_decay=1e-4)
+    if wl.optimizer in ("adamw", "adamw8"):
+        return optim.AdamW(model.parameters(), lr=lr, weight_decay=1e-4, state_bits=8 if wl.optimizer == "adamw8" else 32)
+    if wl.optimizer != "sgd":
+        raise ValueError(f"unknown optimizer {wl.optimizer}")
     return torch.optim.SGD(model.parameters(), lr=lr, weight_decay=0, momentum=0.01)
 
 

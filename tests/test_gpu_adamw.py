@@ -476,3 +476,36 @@ def test_training_of_quantised_layers(ops, optim, bits):
         served = ops.int8_linear(torch.relu(ops.int8_linear(x, w1, a[1])), w2, a[3])
         assert torch.equal(served, ops.int8_linear(torch.relu(ops.int8_linear(x, a[0], a[1])), a[2], a[3]))
     assert ops.int8_status() == 0
+
+
+@pytest.mark.parametrize("name, bits", [("adamw", 32), ("adamw8", 8)])
+def test_optimizer_of_the_training_driver(ops, optim, name, bits):
+    """The optimizer that the training driver makes by name, in a step as the fp16 loop takes it: channels_last model,
+    autocast, loss scaling, gradients in the weights' memory format or not."""
+    import dataclasses
+
+    from rexsc_b200.frontend import train
+
+    wl = dataclasses.replace(train.WORKLOADS["resnet18_or2_L32"], optimizer=name)
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(torch.nn.Conv2d(3, 16, 3), torch.nn.BatchNorm2d(16), torch.nn.ReLU(), torch.nn.Conv2d(16, 8, 3),
+                                torch.nn.Flatten(), torch.nn.Linear(8 * 12 * 12, 10)).cuda().to(memory_format=torch.channels_last)
+    opt = train.make_optimizer(wl, model, lr=1e-3)
+    assert isinstance(opt, optim.AdamW) and isinstance(opt, torch.optim.Optimizer)
+    assert opt.flat_state()["exp_avg"].dtype == (F32 if bits == 32 else torch.float8_e4m3fn)
+    scaler = torch.amp.GradScaler("cuda", init_scale=2.0 ** 10)
+    x = _rand((4, 3, 16, 16), F32, 1).contiguous(memory_format=torch.channels_last)
+    y = torch.randint(0, 10, (4,), device="cuda")
+    before = [p.detach().clone() for p in model.parameters()]
+    for _ in range(3):
+        opt.zero_grad()
+        with torch.autocast("cuda", dtype=F16):
+            loss = torch.nn.functional.cross_entropy(model(x), y)
+        scaler.scale(loss).backward()
+        scaler.step(opt)
+        scaler.update()
+    assert int(opt.flat_state()["step"]) == 3
+    for p, q in zip(model.parameters(), before):
+        assert p.isfinite().all() and not torch.equal(p.detach(), q)
+    with pytest.raises(ValueError):
+        train.make_optimizer(dataclasses.replace(wl, optimizer="rmsprop"), model)

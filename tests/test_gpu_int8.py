@@ -154,6 +154,46 @@ def test_sums_of_products_are_exact(ops, m, n, k, kernel):
     assert torch.equal(y, (a.double() @ b.double().t()).float())
 
 
+@pytest.mark.parametrize("m, n, k", [(2600, 2700, 300), (5000, 600, 1100), (300, 20000, 130), (260, 260, 20000), (40, 300, 40000),
+                                     (20000, 130, 128)])
+def test_many_tiles_and_long_contractions(ops, m, n, k):
+    # more output tiles than CTAs, rings of stages filled many times over, several products' accumulators in turn
+    a = torch.randint(-128, 128, (m, k), generator=_gen(1), device="cuda").to(torch.int8)
+    b = torch.randint(-128, 128, (n, k), generator=_gen(2), device="cuda").to(torch.int8)
+    ma = ops.Int8Matrix.from_values(a, torch.ones(m, device="cuda"))
+    mb = ops.Int8Matrix.from_values(b, torch.ones(n, device="cuda"))
+    ref = (a.double() @ b.double().t()).float()
+    for kernel in ("split", "pair", "auto"):
+        ops.set_int8_kernel(kernel)
+        y = ops.int8_matmul(ma, mb)
+        ops.set_int8_kernel("auto")
+        assert torch.equal(y, ref), kernel
+    assert ops.int8_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n, k", [(1, 1), (130, 9), (300, 128), (1000, 515), (77, 2000), (4096, 4096), (129, 33000)])
+def test_a_few_tokens(ops, n, k, dtype):
+    """Up to 32 tokens are quantised by the product's kernel where they are few values; forcing the other kernel quantises them
+    with a launch of their own.  Both are the same integers and sums."""
+    base = _rand((33, k + 3), dtype, 1)
+    base[4] = 0
+    base[6] = float("nan")
+    base[6, 3] = float("inf")
+    base[9] *= 1e-30 if dtype != F16 else 1e-6
+    w = ops.int8_quantize(_rand((n, k), F32, 2, k ** -0.5))
+    bias = _rand((n,), BF16, 3)
+    for x in (base[:, :k], base[:, 3:], base[:, 1:k + 1].contiguous()):
+        for m in (1, 2, 3, 4, 5, 8, 13, 16, 17, 24, 31, 32, 33):
+            y = ops.int8_linear(x[:m], w, bias)
+            ops.set_int8_kernel("pair")
+            ref = ops.int8_linear(x[:m], w, bias)
+            ops.set_int8_kernel("auto")
+            assert torch.equal(y.nan_to_num(7.0), ref.nan_to_num(7.0)) and torch.equal(y.isnan(), ref.isnan())
+            assert int(y.isnan().any(1).sum()) == (m > 6)
+    assert ops.int8_status() == 0
+
+
 @pytest.mark.parametrize("kernel", ["split", "pair"])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("m, n, k", [(1, 1000, 512), (19, 333, 700), (300, 520, 2050), (513, 1024, 640)])
