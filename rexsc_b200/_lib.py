@@ -119,6 +119,23 @@ def load() -> C.CDLL:
     return lib
 
 
+_host = None
+
+
+def host():
+    """The Python extension for the host's side of some calls (csrc/host.cpp); raises if it has not been built."""
+    global _host
+    if _host is None:
+        if not os.path.exists(os.path.join(HERE, "_host.so")):
+            raise ImportError(f"{os.path.join(HERE, '_host.so')} is missing. Build it first:  python -m rexsc_b200.build")
+        load()
+        import torch  # noqa: F401  (its libraries have to be there before the extension)
+        from . import _host as module
+
+        _host = module
+    return _host
+
+
 def check(rc: int, what: str) -> None:
     if rc == OK:
         return

@@ -806,125 +806,6 @@ def int8_matmul(a: Int8Matrix, b: Int8Matrix, bias: torch.Tensor = None, dtype: 
         return _int8_matmul(a, b, bias, dtype, what)
 
 
-@functools.lru_cache(maxsize=1024)
-def _int8_scratch(m: int, n: int, k: int, kernel: int) -> int:
-    return _lib.load().rexsc_int8_linear_workspace_size(m, n, k, kernel)
-
-
-@functools.lru_cache(maxsize=1024)
-def _int8_bwd_scratch(m: int, n: int, dx: bool, dw: bool, db: bool) -> int:
-    return _lib.load().rexsc_int8_linear_bwd_workspace_size(m, n, dx, dw, db)
-
-
-def _tile_bytes(rows: int, cols: int) -> int:
-    return -(-rows // 128) * -(-cols // 128) * 16384
-
-
-class _Int8Linear(torch.autograd.Function):
-    """y = x w^T + bias with both operands in 8-bit integers; the gradients are products of 8-bit integers too."""
-
-    @staticmethod
-    def forward(ctx, x, weight, prepared, bias):
-        dev = x.device
-        n, k = (weight if prepared is None else prepared).shape
-        xt, lead = x.dtype, x.shape[:-1]
-        x2 = x if len(lead) == 1 and xt in _DTYPES and x.stride(1) == 1 else _rows_of(x, k)
-        m = x2.size(0)
-        ctx.lead = lead
-        ctx.dtypes = xt, None if weight is None else weight.dtype, None if bias is None else bias.dtype
-        ctx.sizes = m, n, k
-        if m == 0:
-            return x2.new_empty((*ctx.lead, n))
-        ctx.kernel = kernel = _int8_kernel()
-        want_x, want_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        with _on(dev):
-            # both quantised operands with their scales; one buffer where the backward pass needs both
-            at_w = _tile_bytes(m, k) + -(-m // 64) * 256
-            nbytes = at_w + (_tile_bytes(n, k) + -(-n // 64) * 256 if prepared is None else 0)
-            buf = torch.empty(nbytes, dtype=torch.int8, device=dev)
-            base = buf.data_ptr()
-            xs = base + _tile_bytes(m, k)
-            if prepared is None:
-                w2 = weight if weight.dtype in _DTYPES and weight.stride(1) == 1 else _rows_of(weight, k)
-                wd, w_ptr, w_dtype, w_stride = base + at_w, w2.data_ptr(), _DTYPES[w2.dtype], w2.stride(0)
-                ws = wd + _tile_bytes(n, k)
-            else:
-                wd, ws, w_ptr, w_dtype, w_stride = prepared.data.data_ptr(), prepared.scale.data_ptr(), 0, 0, 0
-            keep, bias_ptr, bias_dtype = _int8_bias(bias, n, dev, "int8_linear")
-            code = _DTYPES[x2.dtype]
-            y = torch.empty((m, n), dtype=x2.dtype, device=dev)
-            rc = _lib.load().rexsc_int8_linear_train_fwd(x2.data_ptr(), code, m, k, x2.stride(0), w_ptr, w_dtype, n, w_stride,
-                                                         bias_ptr, bias_dtype, base, xs, wd, ws, y.data_ptr(), code, kernel,
-                                                         _stream(dev))
-            if rc:
-                _lib.check(rc, "rexsc_int8_linear_train_fwd")
-            del keep
-            if prepared is not None:
-                kept = (None, prepared.data, prepared.scale)
-            elif want_x and not want_w:     # the activations are not needed again: only the weights stay
-                kept = (buf[at_w:].clone(), None, None)
-            else:
-                kept = (buf, None, None)
-        ctx.save_for_backward(*kept)
-        ctx.at_w = 0 if want_x and not want_w else at_w
-        return y if len(lead) == 1 else y.view(*lead, n)
-
-    @staticmethod
-    def backward(ctx, dy):
-        # (a graph of the backward pass is asked for: its nodes raise when they are used.  The wrapper costs the host 5 us)
-        return _int8_linear_once(ctx, dy) if torch.is_grad_enabled() else _Int8Linear.gradients(ctx, dy)
-
-    @staticmethod
-    def gradients(ctx, dy):
-        m, n, k = ctx.sizes
-        want_dx, want_dw, _, want_db = ctx.needs_input_grad
-        xt, wt, bt = ctx.dtypes
-        dev = dy.device
-        if m == 0:
-            zeros = lambda want, shape, t: torch.zeros(shape, dtype=t, device=dev) if want else None
-            return zeros(want_dx, (*ctx.lead, k), xt), zeros(want_dw, (n, k), wt), None, zeros(want_db, (n,), bt)
-        with _on(dev):
-            buf, wdata, wscale = ctx.saved_tensors
-            xd = xs = wd = ws = 0
-            if buf is not None:
-                base = buf.data_ptr()
-                xd, xs = base, base + _tile_bytes(m, k)
-                wd = base + ctx.at_w
-                ws = wd + _tile_bytes(n, k)
-            if wdata is not None:
-                wd, ws = wdata.data_ptr(), wscale.data_ptr()
-            g = dy if dy.dim() == 2 and dy.dtype in _DTYPES and dy.stride(1) == 1 else _rows_of(dy, n)
-            dx = dw = db = None
-            dx_ptr = dw_ptr = db_ptr = dx_code = dw_code = db_code = 0
-            if want_dx:
-                dx = g.new_empty((m, k), dtype=xt if xt in _DTYPES else torch.float32)
-                dx_ptr, dx_code = dx.data_ptr(), _DTYPES[dx.dtype]
-            if want_dw:
-                dw = g.new_empty((n, k), dtype=wt if wt in _DTYPES else torch.float32)
-                dw_ptr, dw_code = dw.data_ptr(), _DTYPES[dw.dtype]
-            if want_db:
-                db = g.new_empty((n,), dtype=bt if bt in _DTYPES else torch.float32)
-                db_ptr, db_code = db.data_ptr(), _DTYPES[db.dtype]
-            nbytes = _int8_bwd_scratch(m, n, want_dx, want_dw, want_db)
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            rc = _lib.load().rexsc_int8_linear_bwd(g.data_ptr(), _DTYPES[g.dtype], m, n, k, g.stride(0), xd, xs, wd, ws, dx_ptr,
-                                                   dx_code, dw_ptr, dw_code, db_ptr, db_code, ctx.kernel, scratch.data_ptr(),
-                                                   nbytes, _stream(dev))
-            if rc:
-                _lib.check(rc, "rexsc_int8_linear_bwd")
-            if want_dx:
-                dx = dx if len(ctx.lead) == 1 else dx.view(*ctx.lead, k)
-                dx = dx if dx.dtype == xt else dx.to(xt)
-            if want_dw and dw.dtype != wt:
-                dw = dw.to(wt)
-            if want_db and db.dtype != bt:
-                db = db.to(bt)
-            return dx, dw, None, db
-
-
-_int8_linear_once = torch.autograd.function.once_differentiable(_Int8Linear.gradients)
-
-
 @_traced
 def int8_linear(x: torch.Tensor, weight, bias: torch.Tensor = None) -> torch.Tensor:
     """A linear layer in 8-bit integers: ``x`` [..., k] is quantised per token, multiplied with ``weight`` and returned in
@@ -942,49 +823,14 @@ def int8_linear(x: torch.Tensor, weight, bias: torch.Tensor = None) -> torch.Ten
     Both directions can be captured into a CUDA graph; every call has scratch of its own.  As with any op of torch, drop all
     eager graphs of the same leaves (outputs that still hold one) before capturing a backward pass: torch's engine would wait
     on the stream of their leaf nodes, which ends the capture, or the process, with an error."""
-    prepared = type(weight) is Int8Matrix
-    if prepared:
-        n, k, dev = weight.rows, weight.cols, weight.data.device
+    host = _lib._host or _lib.host()
+    if type(weight) is Int8Matrix:
+        y = host.int8_linear(x, None, weight.data, weight.scale, weight.rows, weight.cols, bias, _int8_kernel())
     else:
-        _require_cuda(weight, "int8_linear")
-        if weight.dim() != 2 or not weight.is_floating_point():
-            raise ValueError("int8_linear: expected a floating-point weight [n, k] or an Int8Matrix")
-        (n, k), dev = weight.shape, weight.device
-    if x.device != dev or x.dim() < 1 or x.size(-1) != k or n == 0 or k == 0 or not x.is_floating_point():
-        _require_cuda(x, "int8_linear")
-        if x.device != dev:
-            raise ValueError(f"int8_linear: x is on {x.device}, the weights are on {dev}")
-        raise ValueError(f"int8_linear: expected floating-point x [..., {k}] for weights [{n}, {k}], neither of them 0")
-    if k > _lib.INT8_MAX_DOT:
-        raise ValueError(f"int8_linear: sums of more than {_lib.INT8_MAX_DOT} products are not supported (k = {k})")
-    if torch.is_grad_enabled() and (x.requires_grad or (not prepared and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
-        if x.requires_grad and n > _lib.INT8_MAX_DOT:
-            raise ValueError(f"int8_linear: the gradient of x sums over {n} output channels, at most {_lib.INT8_MAX_DOT}")
-        if not prepared and weight.requires_grad and x.numel() // k > _lib.INT8_MAX_DOT:
-            raise ValueError(f"int8_linear: the weight's gradient sums over {x.numel() // k} tokens, at most "
-                             f"{_lib.INT8_MAX_DOT}")
-        return _Int8Linear.apply(x, None if prepared else weight, weight if prepared else None, bias)
-    with _on(dev):
-        ordinary = x.dim() == 2 and x.dtype in _DTYPES and x.stride(1) == 1
-        x2 = x if ordinary else _rows_of(x, k)
-        m = x2.size(0)
-        keep, bias_ptr, bias_dtype = (None, 0, 0) if bias is None else _int8_bias(bias, n, dev, "int8_linear")
-        out = x2.new_empty((m, n))
-        if m:
-            w = weight if prepared else _int8_quantize(_rows_of(weight, k), "int8_linear")
-            kernel, code = _int8_kernel(), _DTYPES[x2.dtype]
-            nbytes = _int8_scratch(m, n, k, kernel)
-            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-            rc = _lib.load().rexsc_int8_linear_fwd(x2.data_ptr(), code, m, k, x2.stride(0), w.data.data_ptr(),
-                                                   w.scale.data_ptr(), n, bias_ptr, bias_dtype, out.data_ptr(), code, kernel,
-                                                   scratch.data_ptr() if nbytes else 0, nbytes, _stream(dev))
-            if rc:
-                _lib.check(rc, "rexsc_int8_linear_fwd")
-            if _DEBUG:
-                _lib.check(int8_status(dev), "rexsc_int8_linear_fwd (device status)")
-    del keep
-    return out if ordinary else out.view(*x.shape[:-1], n)
+        y = host.int8_linear(x, weight, None, None, 0, 0, bias, _int8_kernel())
+    if _DEBUG:
+        _lib.check(int8_status(y.device), "int8_linear (device status)")
+    return y
 
 
 def int8_status(device=None) -> int:

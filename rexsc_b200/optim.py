@@ -6,11 +6,8 @@ place in ``utils_own.train``: it is a ``torch.optim.Optimizer``, so learning-rat
 """
 from __future__ import annotations
 
-import ctypes as C
-import operator
 from typing import Dict
 
-import numpy as np
 import torch
 
 try:
@@ -20,11 +17,8 @@ except ImportError:  # a torch without hooks for all optimizers
     _PRE_HOOKS, _POST_HOOKS = {}, {}
 
 from . import _lib
-from .ops import _DTYPES, _on, _stream
+from .ops import _DTYPES, _on
 
-_STRIDED = torch.strided
-_stride, _numel, _data_ptr, _dtype = (torch.Tensor.stride, torch.Tensor.numel, torch.Tensor.data_ptr,
-                                      operator.attrgetter("dtype"))
 BLOCK = 256  # elements of a block of the flat moment buffers (of a scale of 8-bit moments)
 
 
@@ -95,8 +89,6 @@ class AdamW(torch.optim.Optimizer):
                         "exp_avg_scale": zeros(first[-1], torch.float32),
                         "exp_avg_sqrt_scale": zeros(first[-1], torch.float32)}
             step = zeros(2, torch.int64)
-        table = np.zeros((len(params), 4), dtype=np.int64)  # rexsc_adamw_tensor: param, grad, numel, first_block
-        table[:, 2], table[:, 3] = sizes, first[:-1]
         for i, p in enumerate(params):
             a, b = first[i] * BLOCK, first[i] * BLOCK + sizes[i]
             views = {}
@@ -106,15 +98,10 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     views[name] = t[a:b].as_strided(p.shape, p.stride()) if b > a else t[a:b].view(p.shape)
             self.state[p] = {"step": step[0], **views}
-        d = _lib.AdamWDesc()
-        d.state_bits = self._state_bits
         second = "exp_avg_sq" if self._state_bits == 32 else "exp_avg_sqrt"
-        d.d_step, d.d_exp_avg, d.d_exp_avg_sq = step.data_ptr(), flat["exp_avg"].data_ptr(), flat[second].data_ptr()
-        if self._state_bits == 8:
-            d.d_exp_avg_scale = flat["exp_avg_scale"].data_ptr()
-            d.d_exp_avg_sq_scale = flat["exp_avg_sqrt_scale"].data_ptr()
-        return {"flat": flat, "step": step, "table": table, "desc": d, "device": dev, "sizes": sizes,
-                "strides": [p.stride() for p in params]}
+        native = _lib.host().AdamWPlan(params, self._state_bits, step, flat["exp_avg"], flat[second], flat.get("exp_avg_scale"),
+                                       flat.get("exp_avg_sqrt_scale"))
+        return {"flat": flat, "step": step, "native": native, "strides": [p.stride() for p in params]}
 
     @staticmethod
     def _check_numbers(group) -> None:
@@ -180,8 +167,12 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        scale, inf = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
         for group, plan in zip(self.param_groups, self._plans):
-            self._step_group(group, plan)
+            lr, (b1, b2) = group["lr"], group["betas"]
+            on_device = isinstance(lr, torch.Tensor) and lr.is_cuda
+            plan["native"].step(group["params"], 0.0 if on_device else float(lr), lr if on_device else None, b1, b2,
+                                group["eps"], group["weight_decay"], scale, inf)
         for hook in (*self._optimizer_step_post_hooks.values(), *_POST_HOOKS.values()):
             hook(self, (self, closure), {})
         return loss
@@ -189,77 +180,6 @@ class AdamW(torch.optim.Optimizer):
     # torch wraps an optimizer's step in a profiler range and calls the hooks there, 10 us of the host's time in a step
     # whose launch takes 4; the hooks are called above instead
     step.hooked = True
-
-    def _gather(self, group, plan):
-        """Parameters that take part in a step, their gradients in the parameters' order of memory, and their places."""
-        params, strides, sizes = group["params"], plan["strides"], plan["sizes"]
-        grads = [p.grad for p in params]
-        # whole lists at a time: a loop over the tensors costs the host twice as much
-        try:
-            ordinary = (list(map(_stride, grads)) == strides and list(map(_numel, grads)) == sizes
-                        and list(map(_stride, params)) == strides and list(map(_numel, params)) == sizes and 0 not in sizes)
-        except (TypeError, RuntimeError):   # a gradient that is None, or has no strides (sparse)
-            ordinary = False
-        if ordinary:
-            return params, grads, plan["table"].copy()
-        chosen, kept = [], []
-        for i, (p, g) in enumerate(zip(params, grads)):
-            if g is None or sizes[i] == 0:
-                continue
-            if p.stride() != strides[i] or p.numel() != sizes[i] or p.device != plan["device"]:
-                raise ValueError("AdamW: a parameter has changed its size, memory format or device")
-            if g.layout is not _STRIDED:
-                raise ValueError("AdamW: sparse gradients are not supported")
-            if g.stride() != strides[i] or g.numel() != sizes[i]:
-                g = torch.empty_strided(p.shape, strides[i], dtype=g.dtype, device=g.device).copy_(g.detach())
-            chosen.append(i)
-            kept.append(g)
-        return [params[i] for i in chosen], kept, plan["table"][chosen]
-
-    def _step_group(self, group, plan) -> None:
-        params, grads, table = self._gather(group, plan)
-        if not params:
-            return
-        kinds = list(zip(map(_dtype, params), map(_dtype, grads)))
-        distinct = set(kinds)
-        for pair in distinct:
-            if pair[0] not in _DTYPES:
-                raise ValueError(f"AdamW: parameters must be float32, float16 or bfloat16 (got {pair[0]})")
-        if any(pair[1] not in _DTYPES for pair in distinct):
-            grads = [g if g.dtype in _DTYPES else g.detach().float() for g in grads]
-            kinds = list(zip(map(_dtype, params), map(_dtype, grads)))
-            distinct = set(kinds)
-        table[:, 0] = list(map(_data_ptr, params))
-        table[:, 1] = list(map(_data_ptr, grads))
-        dev, flat, d = plan["device"], plan["flat"], plan["desc"]
-        d.beta1, d.beta2 = group["betas"]
-        d.eps, d.weight_decay = group["eps"], group["weight_decay"]
-        keep = []
-        lr = group["lr"]
-        if isinstance(lr, torch.Tensor) and lr.is_cuda:
-            keep.append(lr.detach().to(device=dev, dtype=torch.float32))
-            d.d_lr, d.lr = keep[-1].data_ptr(), 0.0
-        else:
-            d.d_lr, d.lr = None, float(lr)
-        d.d_grad_scale = d.d_found_inf = None
-        for name in ("grad_scale", "found_inf"):
-            t = getattr(self, name, None)
-            if t is not None:
-                if t.device != dev or t.dtype is not torch.float32:
-                    t = t.to(device=dev, dtype=torch.float32)
-                keep.append(t)
-                setattr(d, "d_" + name, t.data_ptr())
-        launch = _lib.load().rexsc_adamw_step
-        with _on(dev):
-            stream = _stream(dev)
-            for j, kind in enumerate(distinct):
-                part = table if len(distinct) == 1 else np.ascontiguousarray(table[[k == kind for k in kinds]])
-                d.param_dtype, d.grad_dtype = _DTYPES[kind[0]], _DTYPES[kind[1]]
-                d.advance = j == len(distinct) - 1
-                rc = launch(C.byref(d), part.ctypes.data, len(part), stream)
-                if rc:
-                    _lib.check(rc, "rexsc_adamw_step")
-
 
 def _dense(t: torch.Tensor) -> bool:
     """Whether the elements of a tensor fill a contiguous piece of memory, each its own place."""
