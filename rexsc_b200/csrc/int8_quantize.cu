@@ -183,14 +183,22 @@ grad_amax_kernel(const T *__restrict__ dy, long long m, long long n, long long s
             }
         };
         constexpr int kAhead = 4; // rows of a warp that are loaded together
-        for (long long r = r0 + warp; r < r1; r += 8 * kAhead) {
-            Raw<T> raw[kAhead];
+        long long r = r0 + warp;
+        if (vec && c0 + kGCols <= n) { // (no edge: addresses and bounds are a third of the instructions otherwise)
+            const T *at = dy + r * stride + c;
+            const long long pace = 8 * stride;
+            for (; r + 8 * (kAhead - 1) < r1; r += 8 * kAhead, at += kAhead * pace) {
+                Raw<T> raw[kAhead];
 #pragma unroll
-            for (int j = 0; j < kAhead; j++)
-                if (r + 8 * j < r1) load_raw(dy + (r + 8 * j) * stride, c, n, vec, raw[j]);
+                for (int j = 0; j < kAhead; j++) load_raw(at + j * pace, raw[j]);
 #pragma unroll
-            for (int j = 0; j < kAhead; j++)
-                if (r + 8 * j < r1) take(raw[j], r + 8 * j);
+                for (int j = 0; j < kAhead; j++) take(raw[j], r + 8 * j);
+            }
+        }
+        for (; r < r1; r += 8) {
+            Raw<T> raw;
+            load_raw(dy + r * stride, c, n, vec, raw);
+            take(raw, r);
         }
         if (tile) __syncthreads(); // the tile before has been read
 #pragma unroll
@@ -222,7 +230,8 @@ grad_quantize_kernel(const T *__restrict__ dy, long long m, long long n, long lo
                      float *__restrict__ sg, int8_t *__restrict__ qh, float *__restrict__ sh, B *__restrict__ db)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ float row_a[kI8Tile], row_inv[kI8Tile], row_s[kI8Tile], col_a[kGCols], col_inv[kGCols];
+    __shared__ float row_a[kI8Tile], row_inv[kI8Tile], row_s[kI8Tile];
+    __shared__ __align__(16) float col_a[kGCols], col_inv[kGCols], col_s[kGCols];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned row_block = blockIdx.x / col_blocks, col_block = blockIdx.x - row_block * col_blocks;
     const long long c = (long long)col_block * kGCols + lane * 8, r0 = (long long)row_block * kI8Tile;
@@ -238,6 +247,7 @@ grad_quantize_kernel(const T *__restrict__ dy, long long m, long long n, long lo
         col_inv[threadIdx.x] = live ? inverse_of(__uint_as_float(most)) : 0.f;
         if (row_block == 0 && col < n) sh[col] = most < 0x7f800000u ? __fdiv_rn(__uint_as_float(most), 127.f) : nan;
     }
+    col_s[threadIdx.x] = qg && col < n ? col_scale[col] : 0.f;
     if (db && row_block == 0 && col < n) {
         float s = 0.f;
 #pragma unroll 8
@@ -258,14 +268,14 @@ grad_quantize_kernel(const T *__restrict__ dy, long long m, long long n, long lo
     }
     __syncthreads();
     if (c >= tcols * kI8Tile) return;
-    float cs[8], ci[8];
     bool tiny = false; // a column of this lane whose 127 / a overflows: every value takes the exact way
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        cs[i] = qg && c + i < n ? col_scale[c + i] : 0.f;
-        ci[i] = qh ? col_inv[lane * 8 + i] : 0.f;
-        tiny |= qh && ci[i] == 0.f && col_a[lane * 8 + i] > 0.f;
-    }
+    for (int i = 0; i < 8; i++) tiny |= qh && col_inv[lane * 8 + i] == 0.f && col_a[lane * 8 + i] > 0.f;
+    // (the columns' scales stay in shared memory: in registers they leave no room for the loads ahead)
+    auto eight = [&](const float *from, float (&v)[8]) {
+        const float4 p = *reinterpret_cast<const float4 *>(from + lane * 8), q = *reinterpret_cast<const float4 *>(from + lane * 8 + 4);
+        v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w, v[4] = q.x, v[5] = q.y, v[6] = q.z, v[7] = q.w;
+    };
     // of row 0's chunk, without the swizzle (r0 and the block's first column begin a tile)
     const size_t base = ((size_t)row_block * tcols + (size_t)(c >> 7)) * kI8TileBytes + (size_t)(lane & 1) * 8;
     auto take = [&](const Raw<T> &raw, int row) { // row of the tile
@@ -273,6 +283,8 @@ grad_quantize_kernel(const T *__restrict__ dy, long long m, long long n, long lo
         widen(raw, v);
         const size_t at = base + row * 128 + (((lane >> 1 & 7) ^ (row & 7)) << 4);
         if (qg) {
+            float cs[8];
+            eight(col_s, cs);
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = __fmul_rn(v[i], cs[i]);
             const float a = row_a[row];
@@ -281,7 +293,8 @@ grad_quantize_kernel(const T *__restrict__ dy, long long m, long long n, long lo
         if (qh) {
             const float rs = row_s[row];
             uint32_t q[8];
-            float far = 0.f;
+            float far = 0.f, ci[8];
+            eight(col_inv, ci);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[i] = __fmul_rn(v[i], rs);
@@ -301,18 +314,26 @@ grad_quantize_kernel(const T *__restrict__ dy, long long m, long long n, long lo
             *reinterpret_cast<uint2 *>(qh + at) = make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
         }
     };
-    constexpr int kAhead = 2;
+    const T *at = dy + (r0 + warp) * stride + c;
+    const long long pace = 8 * stride;
+    if (vec && r0 + kI8Tile <= m && (long long)(col_block + 1) * kGCols <= n) {
+        constexpr int kAhead = 4;
 #pragma unroll 1
-    for (int j = 0; j < kI8Tile / 8; j += kAhead) {
-        Raw<T> raw[kAhead];
+        for (int row = warp; row < kI8Tile; row += 8 * kAhead, at += kAhead * pace) {
+            Raw<T> raw[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            const long long r = r0 + (j + i) * 8 + warp;
-            if (r < m) load_raw(dy + r * stride, c, n, vec, raw[i]);
-            else clear_raw(raw[i]);
+            for (int i = 0; i < kAhead; i++) load_raw(at + i * pace, raw[i]);
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) take(raw[i], row + 8 * i);
         }
-#pragma unroll
-        for (int i = 0; i < kAhead; i++) take(raw[i], (j + i) * 8 + warp);
+    } else {
+#pragma unroll 1
+        for (int row = warp; row < kI8Tile; row += 8) {
+            Raw<T> raw;
+            if (r0 + row < m) load_raw(dy + (r0 + row) * stride, c, n, vec, raw);
+            else clear_raw(raw);
+            take(raw, row);
+        }
     }
 }
 
