@@ -137,25 +137,57 @@ template <> __device__ __forceinline__ float narrow<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// eight e4m3 codes (4 exponent bits with bias 7, 3 of mantissa, steps of 2^-9 below 2^-6), times a scale
-__device__ __forceinline__ void from_e4m3(uint2 codes, float scale, float (&v)[8])
+// two fp32 in a register pair; every operation rounds each of them as the scalar one does
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair(float lo, float hi)
 {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ Pair both(float v) { return pair(v, v); }
+__device__ __forceinline__ void apart(Pair p, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ Pair mul2(Pair a, Pair b)
+{
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// (by halves: from a product and an addition of pairs the compiler makes one operation with one rounding, .rn or not)
+__device__ __forceinline__ Pair add2(Pair a, Pair b)
+{
+    float a0, a1, b0, b1;
+    apart(a, a0, a1);
+    apart(b, b0, b1);
+    return pair(__fadd_rn(a0, b0), __fadd_rn(a1, b1));
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c)
+{
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// eight e4m3 codes (4 exponent bits with bias 7, 3 of mantissa, steps of 2^-9 below 2^-6), times a scale
+__device__ __forceinline__ void from_e4m3(uint2 codes, float scale, Pair (&v)[4])
+{
+    const Pair s = both(scale);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t pair = i < 2 ? codes.x : codes.y;
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(i & 1 ? pair >> 16 : pair & 0xffff), __NV_E4M3);
+        const uint32_t two = i < 2 ? codes.x : codes.y;
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(i & 1 ? two >> 16 : two & 0xffff), __NV_E4M3);
         const float2 f = __half22float2(__half2(h));
-        v[2 * i] = __fmul_rn(f.x, scale), v[2 * i + 1] = __fmul_rn(f.y, scale);
+        v[i] = mul2(pair(f.x, f.y), s);
     }
 }
-// y in [0, 448] to e4m3, rounded up by the threshold u / 2^20.  From 2^-6 on the fraction is the low 20 bits of y's mantissa;
-// below, steps are 2^-9 and the fraction that of y * 2^9 plus the threshold, a sum in fp32 whose whole part an addition of
-// 2^23 that rounds down leaves in the low bits.  (Only the low byte counts; its sign bit is 0.)
+// The magnitude of y, at most 448, to e4m3, rounded up by the threshold u / 2^20.  From 2^-6 on the fraction is the low 20 bits
+// of y's mantissa; below, steps are 2^-9 and the fraction that of |y| * 2^9 plus the threshold, a sum in fp32 whose whole part
+// an addition of 2^23 that rounds down leaves in the low bits.  (Only the low byte counts: y's sign does not reach it.)
 __device__ __forceinline__ uint32_t to_e4m3_normal(float y, uint32_t u) { return (__float_as_uint(y) + u - ((127u - 7u) << 23)) >> 20; }
 __device__ __forceinline__ uint32_t to_e4m3_small(float y, uint32_t u)
 {
     const float part = __fadd_rn(__uint_as_float(0x3f800000u | u << 3), -1.f);
-    return __float_as_uint(__fadd_rd(__fmaf_rn(y, 512.f, part), 8388608.f));
+    return __float_as_uint(__fadd_rd(__fmaf_rn(fabsf(y), 512.f, part), 8388608.f));
 }
 // byte `at` of four words
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t at)
@@ -163,19 +195,17 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
     const uint32_t sel = at | (at + 4) << 4;
     return __byte_perm(__byte_perm(a, b, sel), __byte_perm(c, d, sel), 0x5410);
 }
-// Eight magnitudes x, in units whose reciprocal is `per`, as e4m3; least: what is not 0 is not stored as 0.  Blocks whose
-// values all lie above 2^-6 (1 / 28672 of the largest) skip the small steps: 96 -> 50 instructions an element.
-__device__ __forceinline__ uint2 store_e4m3(const float (&x)[8], float most, float per, const uint32_t (&u)[8], bool least)
+// Eight values y in units of a block's scale as e4m3, without their signs; over: the largest of the block is above 448 (by a
+// rounding); least: what is not 0 is not stored as 0.  Blocks whose values all lie above 2^-6 (1 / 28672 of the largest) skip
+// the small steps.
+__device__ __forceinline__ uint2 store_e4m3(float (&y)[8], bool over, const uint32_t (&u)[8], bool least)
 {
-    float y[8], low = 448.f;
+    float low = 448.f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        y[i] = __fmul_rn(fabsf(x[i]), per);
-        low = fminf(low, y[i]);
-    }
-    if (!(__fmul_rn(most, per) <= 448.f)) { // (the same for the block) rounding has put the largest above the largest code
+    for (int i = 0; i < 8; i++) low = fminf(low, fabsf(y[i]));
+    if (over) { // (the same for the block)
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = fminf(y[i], 448.f);
+        for (int i = 0; i < 8; i++) y[i] = fminf(fmaxf(y[i], -448.f), 448.f);
     }
     uint32_t c[8];
 #pragma unroll
@@ -183,11 +213,28 @@ __device__ __forceinline__ uint2 store_e4m3(const float (&x)[8], float most, flo
     if (low < 0x1p-6f) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            if (y[i] < 0x1p-6f) c[i] = to_e4m3_small(y[i], u[i]) & 0xff;
-            if (least && y[i] > 0.f) c[i] = max(c[i], 1u);
+            if (fabsf(y[i]) < 0x1p-6f) c[i] = to_e4m3_small(y[i], u[i]) & 0xff;
+            if (least && fabsf(y[i]) > 0.f) c[i] = max(c[i], 1u);
         }
     }
-    return make_uint2(pack4(c[0], c[1], c[2], c[3], 0), pack4(c[4], c[5], c[6], c[7], 0));
+    return make_uint2(pack4(c[0], c[1], c[2], c[3], 0) & 0x7f7f7f7fu, pack4(c[4], c[5], c[6], c[7], 0) & 0x7f7f7f7fu);
+}
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// Of -v, v > 0, the root's negative: rsqrt's estimate y of 1 / sqrt(v), g = v y, and Newton's step g + (v - g^2) y / 2, whose
+// error before its rounding is below 2^-42 of the root: correctly rounded but where a root lies that near to the middle of
+// two numbers, and then one of them (none of 10^9 random values differed from sqrt.rn, which takes twice the instructions).  For v in [2^-100, 2^126] only.
+__device__ __forceinline__ Pair minus_root(Pair minus_v, float v0, float v1)
+{
+    float y0, y1;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"(v0));
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y1) : "f"(v1));
+    const Pair y = pair(y0, y1), q = mul2(minus_v, y);
+    return fma2(fma2(q, q, minus_v), mul2(y, both(0.5f)), q);
 }
 __device__ __forceinline__ float reciprocal(float x)
 {
@@ -274,41 +321,73 @@ adamw_kernel(const __grid_constant__ AdamLaunch<kList> l)
     auto update = [&](unsigned b, const Block &x) {
         if (x.left < 0) return;
         const size_t pos = (size_t)b * kBlock + lane * 8; // in the flat buffers
-        float p[8], g[8], m[8], v[8];
+        float p[8], g[8];
         widen(x.p, kDtypeOf<P>, p);
         widen(x.g, g_dtype, g);
-        if constexpr (kBits8) {
-            from_e4m3(x.cm, x.sm, m);
-            from_e4m3(x.cr, x.sr, v);
+        auto store_p = [&]() {
+            if (x.vec && x.left == 8) {
+                store8v(x.p_at, p);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = __fmul_rn(v[i], v[i]);
-        } else {
+                for (int i = 0; i < 8; i++)
+                    if (i < x.left) x.p_at[i] = narrow<P>(p[i]);
+            }
+        };
+        // (each operation on the moments is rounded by itself: what is stored in 8 bits is then the same wherever it is
+        //  computed.  The divisor of the weights' change is 0, or neither below 2^-74 nor above 2^84 / sqrt(1 - b2).)
+        if constexpr (!kBits8) {
+            float m[8], v[8];
             load8v(a.m + pos, m);
             load8v(a.v + pos, v);
-        }
-        float r[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            // (each operation rounded by itself: what is stored in 8 bits is then the same wherever it is computed)
-            g[i] = __fmul_rn(g[i], unscale);
-            m[i] = __fadd_rn(__fmul_rn(a.b1, m[i]), __fmul_rn(a.c1, g[i]));
-            v[i] = __fadd_rn(__fmul_rn(a.b2, v[i]), __fmul_rn(a.c2, __fmul_rn(g[i], g[i])));
-            r[i] = __fsqrt_rn(v[i]);
-            // (the divisor is 0, or neither below 2^-74 nor above 2^84 / sqrt(1 - b2))
-            p[i] = fmaf(-size * m[i], reciprocal(fmaf(r[i], root, a.eps)), p[i] * keep);
-        }
-        if (x.vec && x.left == 8) {
-            store8v(x.p_at, p);
+            for (int i = 0; i < 8; i++) {
+                g[i] = __fmul_rn(g[i], unscale);
+                m[i] = __fadd_rn(__fmul_rn(a.b1, m[i]), __fmul_rn(a.c1, g[i]));
+                v[i] = __fadd_rn(__fmul_rn(a.b2, v[i]), __fmul_rn(a.c2, __fmul_rn(g[i], g[i])));
+                p[i] = fmaf(-size * m[i], reciprocal(fmaf(__fsqrt_rn(v[i]), root, a.eps)), p[i] * keep);
+            }
+            store_p();
+            store8v(a.m + pos, m);
+            store8v(a.v + pos, v);
         } else {
+            // two at a time; v and its root with the other sign, which saves the root's step two operations
+            Pair m2[4], r2[4];
+            from_e4m3(x.cm, x.sm, m2);
+            from_e4m3(x.cr, x.sr, r2);
+            uint32_t odd = 0; // how far beyond the range of minus_root
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i < x.left) x.p_at[i] = narrow<P>(p[i]);
-        }
-        if constexpr (kBits8) {
-            uint32_t am = 0, ar = 0; // bits: a NaN is larger than everything
+            for (int i = 0; i < 4; i++) {
+                const Pair gp = mul2(pair(g[2 * i], g[2 * i + 1]), both(unscale));
+                m2[i] = add2(mul2(both(a.b1), m2[i]), mul2(both(a.c1), gp));
+                r2[i] = add2(mul2(both(-a.b2), mul2(r2[i], r2[i])), mul2(both(-a.c2), mul2(gp, gp)));
+                float v0, v1;
+                apart(r2[i], v0, v1);
+                v[2 * i] = -v0, v[2 * i + 1] = -v1;
+                odd = max(odd, max(__float_as_uint(-v0) - 0x0d800000u, __float_as_uint(-v1) - 0x0d800000u)); // 2^-100
+                r2[i] = minus_root(r2[i], -v0, -v1);
+            }
+            if (odd > 0x7e800000u - 0x0d800000u) { // 2^126; zeros and NaN come out above it too
 #pragma unroll
-            for (int i = 0; i < 8; i++) am = max(am, __float_as_uint(m[i]) & 0x7fffffffu), ar = max(ar, __float_as_uint(r[i]));
-            const float most_m = __uint_as_float(__reduce_max_sync(0xffffffffu, am)), most_r = __uint_as_float(__reduce_max_sync(0xffffffffu, ar));
+                for (int i = 0; i < 4; i++) r2[i] = pair(-__fsqrt_rn(v[2 * i]), -__fsqrt_rn(v[2 * i + 1]));
+            }
+            float most_m = 0.f;
+            uint32_t bits_r = 0; // (negative numbers, as bits: the largest magnitude is the largest, a NaN larger still)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float d0, d1, m0, m1, r0, r1;
+                apart(fma2(r2[i], both(-root), both(a.eps)), d0, d1);
+                const Pair pn = fma2(mul2(m2[i], both(-size)), pair(reciprocal(d0), reciprocal(d1)),
+                                     mul2(pair(p[2 * i], p[2 * i + 1]), both(keep)));
+                apart(pn, p[2 * i], p[2 * i + 1]);
+                apart(m2[i], m0, m1);
+                apart(r2[i], r0, r1);
+                most_m = max_nan(max_nan(most_m, fabsf(m0)), fabsf(m1));
+                bits_r = max(bits_r, max(__float_as_uint(r0), __float_as_uint(r1)));
+            }
+            store_p();
+            most_m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_m)));
+            const float most_r = __uint_as_float(__reduce_max_sync(0xffffffffu, bits_r) & 0x7fffffffu);
             // the block's four quotients, one to a lane
             const float most = lane & 1 ? most_r : most_m;
             float quotient = __fdiv_rn(lane & 2 ? most : 448.f, lane & 2 ? 448.f : most);
@@ -318,19 +397,21 @@ adamw_kernel(const __grid_constant__ AdamLaunch<kList> l)
             if (lane == 3) a.rs[b] = quotient;
             const uint32_t u0 = (uint32_t)pos * 0xC13FA9A9u + (uint32_t)t * 0x9E3779B9u;
             uint32_t u[8];
+            float y[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) u[i] = (u0 + i * 0xC13FA9A9u) >> 12;
-            uint2 wm = store_e4m3(m, most_m, per_m, u, false);
-            auto sign = [&](int i) { return __float_as_uint(m[i]); };
-            wm.x |= pack4(sign(0), sign(1), sign(2), sign(3), 3) & 0x80808080u;
-            wm.y |= pack4(sign(4), sign(5), sign(6), sign(7), 3) & 0x80808080u;
+#pragma unroll
+            for (int i = 0; i < 4; i++) apart(mul2(m2[i], both(per_m)), y[2 * i], y[2 * i + 1]);
+            auto sign = [&](int i) { return __float_as_uint(y[i]); };
+            const uint32_t signs0 = pack4(sign(0), sign(1), sign(2), sign(3), 3) & 0x80808080u;
+            const uint32_t signs1 = pack4(sign(4), sign(5), sign(6), sign(7), 3) & 0x80808080u;
+            const uint2 wm = store_e4m3(y, !(__fmul_rn(most_m, per_m) <= 448.f), u, false);
+            *reinterpret_cast<uint2 *>(a.m8 + pos) = make_uint2(wm.x | signs0, wm.y | signs1);
 #pragma unroll
             for (int i = 0; i < 8; i++) u[i] = 0xfffffu - u[i];
-            *reinterpret_cast<uint2 *>(a.m8 + pos) = wm;
-            *reinterpret_cast<uint2 *>(a.r8 + pos) = store_e4m3(r, most_r, per_r, u, true);
-        } else {
-            store8v(a.m + pos, m);
-            store8v(a.v + pos, v);
+#pragma unroll
+            for (int i = 0; i < 4; i++) apart(mul2(r2[i], both(-per_r)), y[2 * i], y[2 * i + 1]);
+            *reinterpret_cast<uint2 *>(a.r8 + pos) = store_e4m3(y, !(__fmul_rn(most_r, per_r) <= 448.f), u, true);
         }
     };
     unsigned b = a.first + blockIdx.x * kWarps + (threadIdx.x >> 5);
