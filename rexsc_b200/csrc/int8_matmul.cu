@@ -837,7 +837,7 @@ int split_of(long long tiles, int k_blocks)
 }
 
 // The kernel that takes less time by what they were measured at (us, B200, bf16): pairs 5.6 + 0.28 for every step of 128 along
-// the contraction and round of 74 output tiles; the split 2 and for every round of 148 CTAs 3 + 0.027 rows and for every step
+// the contraction and wave of 74 output tiles; the split 2 and for every wave of 148 CTAs 3 + 0.027 rows and for every step
 // of a CTA 0.14 + 0.0006 rows.  Whole calls: 1024 x 2048 x 512 pairs 9.9, split 12.3; 512 x 4096 x 4096 18.4 and 18.7;
 // 192 x 8192 x 8192 29.7 and 25.3; 64 x 8192 x 8192 26.0 and 15.6.
 bool use_pairs(const I8Product &p, int kernel)
@@ -846,8 +846,8 @@ bool use_pairs(const I8Product &p, int kernel)
     SplitProblem a;
     const long long tiles = split_shape(&a, p), pairs = ((p.m + 255) / 256) * ((p.n + 255) / 256);
     const int split = split_of(tiles, a.k_blocks);
-    const double rounds = (double)((tiles * split + 147) / 148), steps = (a.k_blocks + split - 1) / split;
-    return 5.6 + (double)((pairs + 73) / 74) * a.k_blocks * 0.28 < 2 + rounds * (3 + 0.027 * a.rows + steps * (0.14 + 0.0006 * a.rows));
+    const double waves = (double)((tiles * split + 147) / 148), steps = (a.k_blocks + split - 1) / split;
+    return 5.6 + (double)((pairs + 73) / 74) * a.k_blocks * 0.28 < 2 + waves * (3 + 0.027 * a.rows + steps * (0.14 + 0.0006 * a.rows));
 }
 
 // stages of a CTA, and the shared memory that it needs

@@ -19,6 +19,18 @@ except ImportError:  # a torch without hooks for all optimizers
 from . import _lib
 from .ops import _DTYPES, _on
 
+class _State(dict):
+    """Per-parameter views of the flat moment buffers, made when they are asked for."""
+
+    def __init__(self, make):
+        super().__init__()
+        self._make = make
+
+    def __missing__(self, p):
+        self[p] = made = self._make(p)
+        return made
+
+
 BLOCK = 256  # elements of a block of the flat moment buffers (of a scale of 8-bit moments)
 
 
@@ -45,7 +57,9 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: state_bits must be 8 or 32 (got {state_bits})")
         self._state_bits = state_bits
         self._plans = []
+        self._place = {}    # parameter -> (its group's plan, its number there)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.state = _State(self._views)
 
     def __getstate__(self):
         raise TypeError("rexsc_b200.optim.AdamW cannot be copied or pickled: use state_dict()")
@@ -53,11 +67,16 @@ class AdamW(torch.optim.Optimizer):
     # -- construction -------------------------------------------------------------------------------------------
     def add_param_group(self, group) -> None:
         super().add_param_group(group)
+        params = self.param_groups[-1]["params"]
         try:
-            self._plans.append(self._plan(self.param_groups[-1]))
+            if len(set(params)) != len(params):
+                raise ValueError("AdamW: a parameter appears twice in its group")
+            plan = self._plan(self.param_groups[-1])
         except Exception:
             self.param_groups.pop()
             raise
+        self._plans.append(plan)
+        self._place.update((p, (plan, i)) for i, p in enumerate(params))
 
     def _plan(self, group) -> dict:
         """Flat moment buffers of a group, every tensor on a block of its own."""
@@ -89,19 +108,22 @@ class AdamW(torch.optim.Optimizer):
                         "exp_avg_scale": zeros(first[-1], torch.float32),
                         "exp_avg_sqrt_scale": zeros(first[-1], torch.float32)}
             step = zeros(2, torch.int64)
-        for i, p in enumerate(params):
-            a, b = first[i] * BLOCK, first[i] * BLOCK + sizes[i]
-            views = {}
-            for name, t in flat.items():
-                if name.endswith("_scale"):
-                    views[name] = t[first[i]:first[i + 1]]
-                else:
-                    views[name] = t[a:b].as_strided(p.shape, p.stride()) if b > a else t[a:b].view(p.shape)
-            self.state[p] = {"step": step[0], **views}
         second = "exp_avg_sq" if self._state_bits == 32 else "exp_avg_sqrt"
         native = _lib.host().AdamWPlan(params, self._state_bits, step, flat["exp_avg"], flat[second], flat.get("exp_avg_scale"),
                                        flat.get("exp_avg_sqrt_scale"))
-        return {"flat": flat, "step": step, "native": native, "strides": [p.stride() for p in params]}
+        return {"flat": flat, "step": step, "native": native, "first": first, "shapes": [p.shape for p in params],
+                "strides": [p.stride() for p in params]}
+
+    def _views(self, p) -> Dict[str, torch.Tensor]:
+        plan, i = self._place[p]
+        first, last, shape, stride = plan["first"][i], plan["first"][i + 1], plan["shapes"][i], plan["strides"][i]
+        views = {"step": plan["step"][0]}
+        for name, t in plan["flat"].items():
+            if name.endswith("_scale"):
+                views[name] = t[first:last]
+            else:
+                views[name] = t.as_strided(shape, stride, first * BLOCK) if last > first else t[:0].view(shape)
+        return views
 
     @staticmethod
     def _check_numbers(group) -> None:
@@ -127,6 +149,8 @@ class AdamW(torch.optim.Optimizer):
     def state_dict(self):
         """As torch's optimizers give it; the tensors are the optimizer's own.  Moments in 8 bits are stored in the order of
         the weights' memory."""
+        for p in self._place:
+            self.state[p]
         sd = super().state_dict()
         sd["state_bits"] = self._state_bits
         for i, (strides, plan) in enumerate((p["strides"], p) for p in self._plans):

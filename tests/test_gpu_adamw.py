@@ -406,6 +406,8 @@ def test_step_refusals(optim):
     with pytest.raises(ValueError):
         opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3))]})
     assert len(opt.param_groups) == 1
+    with pytest.raises(ValueError), pytest.warns(UserWarning):
+        optim.AdamW([p, p])
     p.grad = torch.ones(4, 4, device="cuda")
     p.data = torch.zeros(8, 4, device="cuda")[::2]
     with pytest.raises(ValueError):
@@ -428,6 +430,37 @@ def test_step_refusals(optim):
     import copy
     with pytest.raises(TypeError):
         copy.deepcopy(opt)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_than_2_to_the_31_elements(optim, bits):
+    n = 2 ** 31 + 2 ** 20 + 77
+    p = torch.nn.Parameter(torch.zeros(n, dtype=BF16, device="cuda"))
+    q = torch.nn.Parameter(torch.zeros(300, dtype=BF16, device="cuda"))
+    p.grad = torch.zeros(n, dtype=BF16, device="cuda")
+    tail = 1000
+    with torch.no_grad():
+        p[-tail:] = _rand((tail,), BF16, 1)
+    p.grad[-tail:] = _rand((tail,), BF16, 2)
+    q.grad = _rand((300,), BF16, 3)
+    opt = _make(optim, [p, q], bits)
+    # the tail's blocks as a tensor of its own that begins at the same place
+    start = (n - tail) // 256 * 256
+    ref_p = torch.zeros(n - start, dtype=BF16, device="cuda")
+    ref_p[-tail:] = p.detach()[-tail:]
+    ref, ref_q = Ref(ref_p, bits, start), Ref(q, bits, -(-n // 256) * 256)
+    g = torch.zeros(n - start, device="cuda")
+    g[-tail:] = p.grad[-tail:].float()
+    ref.step(g)
+    ref_q.step(q.grad)
+    opt.step()
+    _check_p(p.detach()[start:], ref)
+    _check_p(q, ref_q)
+    s = opt.state[p]
+    if bits == 8:
+        assert torch.equal(s["exp_avg"][start:].double(), ref.m8.view(-1)[:n - start])
+        assert torch.equal(s["exp_avg_sqrt_scale"][start // 256:].double(), ref.rs.view(-1))
+    assert not s["exp_avg"][:start].view(torch.uint8).any() and not p.detach()[:start].any()
 
 
 # ---- the operators together -------------------------------------------------------------------------------------

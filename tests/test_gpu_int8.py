@@ -367,6 +367,21 @@ def test_gradients_of_broadcast_and_shared_tensors(ops):
     _check(wt.grad.t(), rw)
 
 
+def test_types_beyond_the_kernels(ops):
+    # float64 operands are computed as float32; their gradients come back in float64
+    x, w = _rand((20, 64)).double().requires_grad_(), _rand((30, 64), F32, 1).double().requires_grad_()
+    b = _rand((30,), F32, 2).double().requires_grad_()
+    y = ops.int8_linear(x, w, b)
+    dy = _rand((20, 30), F32, 3)
+    y.backward(dy)
+    assert y.dtype == F32 and x.grad.dtype == w.grad.dtype == b.grad.dtype == torch.float64
+    rx, rw, _, _ = _grads_ref(x.detach().float(), w.detach().float(), dy)
+    _check(x.grad.float(), rx)
+    _check(w.grad.float(), rw)
+    with torch.inference_mode():
+        assert torch.equal(ops.int8_linear(x, w, b), y.detach())
+
+
 def test_gradients_of_odd_batches(ops):
     w, b = _rand((30, 64), F32, 1).requires_grad_(), _rand((30,), F32, 1).requires_grad_()
     x = torch.zeros(0, 64, device="cuda", requires_grad=True)
