@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/rexsc_b200.h"
@@ -35,6 +36,15 @@ void check(int rc, const char *what)
                                                    : "error";
     TORCH_CHECK_VALUE(rc != REXSC_E_BAD_ARG && rc != REXSC_E_UNSUPPORTED && rc != REXSC_E_TOO_LONG, what, ": ", name);
     TORCH_CHECK(false, what, ": ", name, rc == REXSC_E_CUDA ? ": " : "", rc == REXSC_E_CUDA ? rexsc_last_cuda_error() : "");
+}
+
+// Whether two sets of strides put the elements of a tensor in the same places (those of dimensions of one element do not matter)
+bool same_places(at::IntArrayRef sizes, at::IntArrayRef a, at::IntArrayRef b)
+{
+    if (sizes.size() != a.size() || a.size() != b.size()) return false;
+    for (size_t i = 0; i < a.size(); i++)
+        if (sizes[i] != 1 && a[i] != b[i]) return false;
+    return true;
 }
 
 void *stream_of(const at::Device &d) { return c10::cuda::getCurrentCUDAStream(d.index()).stream(); }
@@ -192,6 +202,11 @@ Tensor int8_linear(const Tensor &x, const std::optional<Tensor> &weight_, const 
         TORCH_CHECK_VALUE(weight.dim() == 2 && weight.is_floating_point(),
                           "int8_linear: expected a floating-point weight [n, k] or an Int8Matrix");
         n = weight.size(0), k = weight.size(1);
+    } else {
+        TORCH_CHECK_VALUE(n > 0 && k > 0 && data.is_cuda() && data.scalar_type() == at::kChar && data.is_contiguous() &&
+                              data.numel() >= tile_bytes(n, k) && scale.defined() && scale.device() == data.device() &&
+                              scale.scalar_type() == at::kFloat && scale.is_contiguous() && scale.numel() >= n,
+                          "int8_linear: an Int8Matrix whose data or scale does not fit its size");
     }
     const at::Device dev = (prepared ? data : weight).device();
     TORCH_CHECK_VALUE(x.device() == dev, "int8_linear: x is on ", x.device(), ", the weights are on ", dev);
@@ -270,10 +285,11 @@ public:
     {
         at::NoGradGuard no_grad;
         c10::cuda::CUDAGuard guard(device_);
-        std::vector<Tensor> kept;
+        std::vector<Tensor> kept, changed;
         std::vector<rexsc_adamw_tensor> table;
         std::vector<int> kinds;
         table.reserve(params.size());
+        changed.reserve(params.size());
         kinds.reserve(params.size());
         TORCH_CHECK_VALUE(params.size() == shapes_.size(), "AdamW: a parameter group has changed");
         for (size_t i = 0; i < params.size(); i++) {
@@ -281,20 +297,23 @@ public:
             const Shape &s = shapes_[i];
             Tensor g = p.grad();
             if (!g.defined() || s.numel == 0) continue;
-            TORCH_CHECK_VALUE(p.layout() == at::kStrided && p.numel() == s.numel && p.strides() == at::IntArrayRef(s.strides) &&
+            TORCH_CHECK_VALUE(p.layout() == at::kStrided && p.numel() == s.numel && same_places(p.sizes(), p.strides(), s.strides) &&
                                   p.device() == device_,
                               "AdamW: a parameter has changed its size, memory format or device");
             const int p_code = code_of(p.scalar_type());
             TORCH_CHECK_VALUE(p_code >= 0, "AdamW: parameters must be float32, float16 or bfloat16 (got ", p.scalar_type(), ")");
             TORCH_CHECK_VALUE(g.layout() == at::kStrided, "AdamW: sparse gradients are not supported");
             if (code_of(g.scalar_type()) < 0) g = g.to(at::kFloat);
-            if (g.strides() != at::IntArrayRef(s.strides) || g.numel() != s.numel || g.device() != device_)
+            if (!same_places(p.sizes(), g.strides(), s.strides) || g.sizes() != p.sizes() || g.device() != device_)
                 g = at::empty_strided(p.sizes(), s.strides, g.options().device(device_)).copy_(g);
             table.push_back({p.data_ptr(), g.data_ptr(), s.numel, s.first});
             kinds.push_back(p_code * 4 + code_of(g.scalar_type()));
             kept.push_back(std::move(g)); // (until the launch is on the stream)
+            changed.push_back(p);
         }
         if (table.empty()) return;
+        // autograd knows of writes by their versions: a graph that still needs the old weights raises instead of reading new ones
+        for (const Tensor &p : changed) torch::autograd::impl::bump_version(p);
         rexsc_adamw_desc d = d_;
         const auto scalar = [&](const std::optional<Tensor> &t) -> const float * {
             if (!t) return nullptr;

@@ -687,12 +687,33 @@ def _int8_kernel() -> int:
 class Int8Matrix:
     """A matrix in 8-bit integers with an fp32 scale per row, as :func:`int8_quantize` makes it: row r stands for
     ``values()[r] * scale[r]``.  ``data`` holds the integers in the library's own layout; keep the object as the prepared
-    weights of a layer and build a new one after the weights change."""
+    weights of a layer and build a new one after the weights change.  Its attributes cannot be set; it can be copied and
+    pickled."""
 
     __slots__ = ("rows", "cols", "data", "scale")
 
     def __init__(self, rows: int, cols: int, data: torch.Tensor, scale: torch.Tensor):
-        self.rows, self.cols, self.data, self.scale = rows, cols, data, scale
+        _require_cuda(data, "Int8Matrix")
+        nbytes = _lib.load().rexsc_int8_data_size(rows, cols)
+        if (nbytes == 0 or data.dtype != torch.int8 or data.numel() != nbytes or not data.is_contiguous()
+                or data.data_ptr() % 256):
+            raise ValueError(f"Int8Matrix: expected {nbytes} contiguous bytes of data on 256 for {rows} x {cols}")
+        if (scale.device != data.device or scale.dtype != torch.float32 or tuple(scale.shape) != (rows,)
+                or not scale.is_contiguous()):
+            raise ValueError(f"Int8Matrix: expected a contiguous float32 scale [{rows}] on {data.device}")
+        for name, value in zip(self.__slots__, (rows, cols, data, scale)):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError("Int8Matrix: its attributes cannot be set")
+
+    def _check(self, what: str) -> None:
+        """(tensors can be resized in place)"""
+        if self.data.numel() < _lib.load().rexsc_int8_data_size(self.rows, self.cols) or self.scale.numel() < self.rows:
+            raise ValueError(f"{what}: an Int8Matrix whose data or scale does not fit its size")
+
+    def __reduce__(self):
+        return Int8Matrix, (self.rows, self.cols, self.data, self.scale)
 
     @property
     def shape(self) -> Tuple[int, int]:
@@ -721,6 +742,7 @@ class Int8Matrix:
 
     def values(self) -> torch.Tensor:
         """The integers, int8 [rows, cols]."""
+        self._check("Int8Matrix.values")
         dev = self.data.device
         with _on(dev):
             out = torch.empty((self.rows, self.cols), dtype=torch.int8, device=dev)
@@ -802,6 +824,8 @@ def int8_matmul(a: Int8Matrix, b: Int8Matrix, bias: torch.Tensor = None, dtype: 
         raise ValueError(f"{what}: operands differ in columns ({a.cols}, {b.cols}) or device ({a.device}, {b.device})")
     if dtype not in _DTYPES:
         raise ValueError(f"{what}: dtype must be float32, float16 or bfloat16")
+    a._check(what)
+    b._check(what)
     with _on(a.device):
         return _int8_matmul(a, b, bias, dtype, what)
 

@@ -19,6 +19,7 @@ except ImportError:  # a torch without hooks for all optimizers
 from . import _lib
 from .ops import _DTYPES, _on
 
+
 class _State(dict):
     """Per-parameter views of the flat moment buffers, made when they are asked for."""
 
@@ -71,6 +72,7 @@ class AdamW(torch.optim.Optimizer):
         try:
             if len(set(params)) != len(params):
                 raise ValueError("AdamW: a parameter appears twice in its group")
+            self._check_apart()
             plan = self._plan(self.param_groups[-1])
         except Exception:
             self.param_groups.pop()
@@ -124,6 +126,14 @@ class AdamW(torch.optim.Optimizer):
             else:
                 views[name] = t.as_strided(shape, stride, first * BLOCK) if last > first else t[:0].view(shape)
         return views
+
+    def _check_apart(self) -> None:
+        """One launch updates all tensors at once: no two of them may hold the same element."""
+        spans = sorted((p.device.index or 0, p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
+                       for g in self.param_groups for p in g["params"] if p.is_cuda and p.numel())
+        for (dev, _, end), (next_dev, begin, _) in zip(spans, spans[1:]):
+            if dev == next_dev and begin < end:
+                raise ValueError("AdamW: two parameters share memory")
 
     @staticmethod
     def _check_numbers(group) -> None:
@@ -204,6 +214,7 @@ class AdamW(torch.optim.Optimizer):
     # torch wraps an optimizer's step in a profiler range and calls the hooks there, 10 us of the host's time in a step
     # whose launch takes 4; the hooks are called above instead
     step.hooked = True
+
 
 def _dense(t: torch.Tensor) -> bool:
     """Whether the elements of a tensor fill a contiguous piece of memory, each its own place."""

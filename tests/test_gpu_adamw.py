@@ -542,3 +542,46 @@ def test_optimizer_of_the_training_driver(ops, optim, name, bits):
         assert p.isfinite().all() and not torch.equal(p.detach(), q)
     with pytest.raises(ValueError):
         train.make_optimizer(dataclasses.replace(wl, optimizer="rmsprop"), model)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_counts_as_a_write(optim, bits):
+    """A graph that still needs the weights of before a step raises, as after any write in place."""
+    p, q, still = (torch.nn.Parameter(_rand((300,), seed=i)) for i in range(3))
+    opt = optim.AdamW([p, q, still], state_bits=bits)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    later, other = (p * p).sum(), (still * still).sum()
+    versions = p._version, q._version, still._version
+    opt.step()
+    assert p._version > versions[0] and q._version > versions[1] and still._version == versions[2]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        later.backward()
+    other.backward()
+
+
+def test_parameters_that_share_memory(optim):
+    flat = torch.zeros(1000, device="cuda")
+    halves = [torch.nn.Parameter(flat[:500]), torch.nn.Parameter(flat[500:])]
+    opt = optim.AdamW(halves)
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [torch.nn.Parameter(flat[499:501])]})
+    assert len(opt.param_groups) == 1
+    with pytest.raises(ValueError):
+        optim.AdamW([torch.nn.Parameter(flat), torch.nn.Parameter(flat.view(10, 100))])
+    for p in halves:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert (flat == flat[0]).all() and flat[0] != 0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_strides_of_single_elements_do_not_matter(optim, bits):
+    """The same places with other strides where a dimension has one element: no new layout, for weights and for gradients."""
+    a, b = (torch.nn.Parameter(_rand((6, 1, 3, 3))) for _ in range(2))
+    oa, ob = optim.AdamW([a], state_bits=bits), optim.AdamW([b], state_bits=bits)
+    a.grad, b.grad = _rand((6, 1, 3, 3), seed=1), _rand((6, 1, 3, 3), seed=1).as_strided((6, 1, 3, 3), (9, 1, 3, 1))
+    b.data = b.data.as_strided((6, 1, 3, 3), (9, 1, 3, 1))
+    assert a.stride() != b.stride()
+    oa.step()
+    ob.step()
+    assert torch.equal(a, b)

@@ -517,3 +517,38 @@ def test_refusals(ops):
     with pytest.raises(RuntimeError):   # no second derivative
         g, = torch.autograd.grad(y.sum(), y.grad_fn.next_functions[0][0].variable, create_graph=True)
         g.sum().backward()
+
+
+def test_matrices_that_do_not_fit_their_size_are_refused(ops):
+    """Nothing is launched: each is refused when it is made, or by the check of the call."""
+    m = ops.int8_quantize(_rand((200, 300)))
+    for rows, cols, data, scale in [(200, 300, m.data[:-1], m.scale), (200, 400, m.data, m.scale), (0, 300, m.data, m.scale),
+                                    (200, 300, m.data.float(), m.scale), (200, 300, m.data, m.scale[:-1]),
+                                    (200, 300, m.data, m.scale.double()), (200, 300, m.data, m.scale.cpu()),
+                                    (200, 300, torch.cat([m.data, m.data])[16:16 + m.data.numel()], m.scale),
+                                    (200, 300, m.data, torch.stack([m.scale, m.scale], 1)[:, 0])]:
+        with pytest.raises(ValueError):
+            ops.Int8Matrix(rows, cols, data, scale)
+    with pytest.raises(RuntimeError):
+        ops.Int8Matrix(200, 300, m.data.cpu(), m.scale)
+    for name in ("rows", "cols", "data", "scale"):
+        with pytest.raises(AttributeError):
+            setattr(m, name, getattr(m, name))
+    gone = ops.int8_quantize(_rand((200, 300)))
+    gone.data.resize_(16)
+    with pytest.raises(ValueError):
+        ops.int8_linear(_rand((4, 300)), gone)
+    with pytest.raises(ValueError):
+        ops.int8_matmul(gone, gone)
+    with pytest.raises(ValueError):
+        gone.values()
+
+
+def test_copies_of_a_matrix(ops):
+    import copy
+    import pickle
+
+    m, x = ops.int8_quantize(_rand((200, 300))), _rand((5, 300), seed=1)
+    y = ops.int8_linear(x, m)
+    for other in (copy.deepcopy(m), copy.copy(m), pickle.loads(pickle.dumps(m)), ops.Int8Matrix(200, 300, m.data.clone(), m.scale.clone())):
+        assert other.shape == (200, 300) and torch.equal(ops.int8_linear(x, other), y)
