@@ -18,7 +18,9 @@
 // to carry.  r' > 0 is never stored as 0: a later step would divide by eps alone.  A block whose largest value is below
 // 2^-100 is stored as zeros.  A gradient that is no finite number makes its element's moments so, and in 8 bits its block's.
 //
-// What bounds it: memory.  Per element 28 bytes (fp32 weights and gradients, 32-bit moments), 16 with 8-bit moments.
+// What bounds it.  32-bit moments: memory, 28 bytes an element with fp32 weights and gradients (134M bf16 gradients on fp32
+// weights in 531 us, 6.57 TB/s).  8-bit moments: arithmetic; 16 bytes an element, or 10 with bf16 weights and gradients, would
+// take 206 us for 134M of those, and 54 instructions an element take 305.
 #include <cuda_fp8.h>
 #include <math.h>
 #include <type_traits>
@@ -227,7 +229,8 @@ __device__ __forceinline__ float max_nan(float a, float b)
 }
 // Of -v, v > 0, the root's negative: rsqrt's estimate y of 1 / sqrt(v), g = v y, and Newton's step g + (v - g^2) y / 2, whose
 // error before its rounding is below 2^-42 of the root: correctly rounded but where a root lies that near to the middle of
-// two numbers, and then one of them (none of 10^9 random values differed from sqrt.rn, which takes twice the instructions).  For v in [2^-100, 2^126] only.
+// two numbers, and then one of them (none of 10^9 random values differed from sqrt.rn, which takes twice the instructions).
+// For v in [2^-100, 2^126] only.
 __device__ __forceinline__ Pair minus_root(Pair minus_v, float v0, float v1)
 {
     float y0, y1;

@@ -6,11 +6,13 @@
 //
 // Two kernels:
 //   product_pair_kernel  pairs of CTAs (cta_group::2) on 256 x 256 output tiles, persistent, two accumulators per CTA so that
-//                        the epilogue of a tile runs under the next one's products.
+//                        the epilogue of a tile runs under the next one's products.  Bound by the tensor pipe: 8192^3 in
+//                        333 us (3.30 POP/s), 8192 x 4096 x 4096 in 85 us (3.24).
 //   product_split_kernel 128 columns of the output (lanes of TMEM) x 16 to 128 rows per CTA; the CTAs of a cluster split the
 //                        contraction and join their int32 sums through distributed shared memory (whole numbers: the
 //                        order does not matter).  It takes two products in one launch (a layer's two gradients), and up
-//                        to 32 tokens as they are, which it quantises itself.
+//                        to 32 tokens as they are, which it quantises itself.  Bound by latencies in a row: one token
+//                        through 4096 x 4096 in 8.6 us, of which the weights' 17 MB take 2.6.
 // Every mbarrier wait is bounded; a CTA whose wait gives up raises the library's status word (rexsc_int8_status), stores
 // nothing more, waits for its copies in flight, frees its TMEM and leaves.
 #include <atomic>

@@ -10,7 +10,9 @@ constexpr int kQThreads = 256;
 
 // kWarps warps (1, 2, 4 or 8) have a row; four chunks of eight values per lane stay in registers between the pass for the
 // largest magnitude and the one that quantises, columns beyond those are read twice.  Fewer values per lane would leave the
-// row's own work (its division, addresses and the exchange between its warps) as long as the values'.
+// row's own work (its division, addresses and the exchange between its warps) as long as the values'.  Bound by memory latency
+// at the 32 warps an SM that 64 registers leave: bf16 8192 x 8192 in 40 us (5.0 TB/s), 8192 x 4096 in 22 us; the arithmetic on
+// pairs of values saves a tenth of the instructions and no time.
 constexpr int kChunks = 4;
 template <typename T, int kWarps>
 __global__ void __launch_bounds__(kQThreads, sizeof(T) == 4 ? 3 : 4)
@@ -135,7 +137,9 @@ unsigned blocks_for(long long items)
 // g[m, n] = fl32(dy[m, n] col_scale[n]) is quantised by rows, h[m, n] = fl32(dy[m, n] row_scale[m]) by columns: each folds
 // in the scales of the operand whose rows its contraction runs over.  Two passes over dy: in the first every block leaves the
 // largest magnitudes of its rows and columns and their sums, for the bias; the second joins those (no atomics and nothing to
-// clear) and quantises.  Up to about 100 MB of dy the second pass finds it in L2.
+// clear) and quantises.  Up to about 100 MB of dy the second pass finds it in L2.  8192 x 4096 bf16: 22 and 39 us (67 MB read,
+// 67 MB read and 67 MB written), bound by latency with half the warps an SM could hold: 64 registers a thread; at 48 or 80 the
+// second pass takes 53 and 47 us.  Arithmetic on pairs of values saves instructions here too, and no time.
 constexpr int kGCols = 256;  // columns of a tile of the first pass: a warp has a row of it, eight columns a lane
 
 // max that lets a NaN through
@@ -354,8 +358,9 @@ namespace {
 bool known_dtype(int d) { return d == REXSC_F32 || d == REXSC_F16 || d == REXSC_BF16; }
 
 // Blocks of the first pass.  They follow from the sizes alone: the bias's sum has one order.  Rows: long enough that a block's
-// end is a small part, as long as every SM gets two blocks, and in 128 parts at the most (up to half a million rows); columns in 16 parts at the most
-// (the second pass joins them in every block).
+// end is a small part, as long as every SM gets two blocks, and in 128 parts at the most (up to half a million rows); columns
+// in 16 parts at the most (the second pass joins them in every block).  8192 x 4096 bf16, both passes: blocks of 64 rows
+// 76 us, 128 rows 68, 256 rows 62, 448 rows 68.
 struct GradBlocks {
     int rows, tiles, row_blocks, col_blocks;
     GradBlocks(long long m, long long n)
