@@ -19,13 +19,13 @@
 // 2^-100 is stored as zeros.  A gradient that is no finite number makes its element's moments so, and in 8 bits its block's.
 //
 // What bounds it.  32-bit moments: memory, 28 bytes an element with fp32 weights and gradients (134M bf16 gradients on fp32
-// weights in 531 us, 6.57 TB/s).  8-bit moments: arithmetic; 16 bytes an element, or 10 with bf16 weights and gradients, would
-// take 206 us for 134M of those, and 54 instructions an element take 305.
+// weights in 530 us, 6.58 TB/s).  8-bit moments: arithmetic; 16 bytes an element, or 10 with bf16 weights and gradients, would
+// take 206 us for 134M of those, and 54 instructions an element take 300.
 #include <cuda_fp8.h>
 #include <math.h>
 #include <type_traits>
 
-#include "common.cuh"
+#include "int8.cuh"
 
 namespace rexsc {
 
@@ -252,6 +252,7 @@ __global__ void __launch_bounds__(kThreadsOf<kBits8>, kCtasOf<kBits8>)
 adamw_kernel(const __grid_constant__ AdamLaunch<kList> l)
 {
     const AdamArgs &a = l.a;
+    wait_previous_launch(); // (the next one does not begin before this one's end: it may read weights before it waits)
     if (a.found_inf && *a.found_inf != 0.f) return;
     const int lane = threadIdx.x & 31;
     const long long t = a.step[0] + 1;
@@ -459,17 +460,15 @@ int launch_list(const AdamArgs &a, const rexsc_adamw_tensor *list, cudaStream_t 
         AdamLaunch<kSmallList> l;
         l.a = a;
         fill(l.t);
-        if (same) adamw_kernel<P, kBits8, true, kSmallList><<<grid, kThreads, 0, st>>>(l);
-        else adamw_kernel<P, kBits8, false, kSmallList><<<grid, kThreads, 0, st>>>(l);
+        return launch_under("adamw_kernel", same ? adamw_kernel<P, kBits8, true, kSmallList> : adamw_kernel<P, kBits8, false, kSmallList>,
+                            grid, kThreads, 0, st, l);
     } else {
         AdamLaunch<kLargeList> l;
         l.a = a;
         fill(l.t);
-        if (same) adamw_kernel<P, kBits8, true, kLargeList><<<grid, kThreads, 0, st>>>(l);
-        else adamw_kernel<P, kBits8, false, kLargeList><<<grid, kThreads, 0, st>>>(l);
+        return launch_under("adamw_kernel", same ? adamw_kernel<P, kBits8, true, kLargeList> : adamw_kernel<P, kBits8, false, kLargeList>,
+                            grid, kThreads, 0, st, l);
     }
-    REXSC_LAUNCH_CHECK("adamw_kernel");
-    return REXSC_OK;
 }
 
 } // namespace

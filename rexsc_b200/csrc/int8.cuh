@@ -28,6 +28,40 @@ __device__ __forceinline__ size_t i8_offset(long long r, long long c, long long 
            (size_t)(((((int)c >> 4) & 7) ^ ((int)r & 7)) << 4) + (size_t)(c & 15);
 }
 
+// ---- launches that begin under the end of the one before them on their stream ----------------------------------
+// What keeps them in order:
+//   * a kernel waits for the launch before it (wait_previous_launch) before it touches global memory; only products read
+//     weights that were quantised earlier sooner;
+//   * it lets the next one begin (allow_next_launch) after that wait, and after it has taken its TMEM: when a kernel begins,
+//     all but the launch right before it has finished, the one that wrote those weights too, and a kernel that holds TMEM
+//     while it waits keeps none from the one it waits for.
+// One token through 4096 x 4096, call after call: 8.4 us, 10.2 without.
+__device__ __forceinline__ void wait_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void allow_next_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <typename... P, typename... A>
+int launch_under(const char *what, void (*kernel)(P...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t st, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    note_kernel_launch();
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        set_cuda_error(e, what);
+        return REXSC_E_CUDA;
+    }
+    return REXSC_OK;
+}
+
 // ---- host launchers ------------------------------------------------------------------------------------------
 int launch_i8_quantize_rows(const void *d_x, int dtype, long long rows, long long cols, long long stride, int8_t *d_data,
                             float *d_scale, bool pad_rows, cudaStream_t st);

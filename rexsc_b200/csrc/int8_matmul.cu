@@ -12,7 +12,7 @@
 //                        contraction and join their int32 sums through distributed shared memory (whole numbers: the
 //                        order does not matter).  It takes two products in one launch (a layer's two gradients), and up
 //                        to 32 tokens as they are, which it quantises itself.  Bound by latencies in a row: one token
-//                        through 4096 x 4096 in 8.6 us, of which the weights' 17 MB take 2.6.
+//                        through 4096 x 4096 in 7.8 us, of which the weights' 17 MB take 2.6.
 // Every mbarrier wait is bounded; a CTA whose wait gives up raises the library's status word (rexsc_int8_status), stores
 // nothing more, waits for its copies in flight, frees its TMEM and leaves.
 #include <atomic>
@@ -100,7 +100,6 @@ __device__ __forceinline__ uint32_t cluster_rank()
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void wait_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Shared-memory matrix descriptor, 128-byte swizzle.  Both ways of reading a tile share it: rows 128 bytes apart in groups of
 // 8 that are 1024 bytes apart.  K-major the rows are the operand's rows and 32 products are 32 bytes further; MN-major the
@@ -302,6 +301,8 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
     wait_previous_launch();
+    // (the next launch begins when this one ends: its blocks would crowd on the SMs that have no tile here, 1537 x 1111 x 2049
+    //  in training 78 us so, 72 us as it is)
 
     // stage and its phase, advanced together: a division in these loops costs as much as a copy
     struct Ring {
@@ -520,6 +521,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
     const uint32_t tokens0 = smem0 + a.stages * stage_bytes; // the quantised tokens, [128 columns][rows][128 bytes]
     const int early = nk < a.stages ? nk : a.stages;
 
+    if (kTokens) wait_previous_launch(); // (it may be the one that quantises the weights)
     const int8_t *pw = a.p.b.data + ((size_t)(tj * a.p.b.step_mn) + (size_t)(k0 * a.p.b.step_k)) * kI8TileBytes;
     const size_t step_w = (size_t)a.p.b.step_k * kI8TileBytes;
     if (warp == 0) {
@@ -529,7 +531,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
-        // the weights depend neither on the tokens nor on the launch before, which quantises the rows: begin with them
+        // the weights depend neither on the tokens nor, where that quantises the rows, on the launch before: begin with them
         for (int s = 0; s < early; s++) {
             mbar_expect_one(full(s), stage_bytes);
             copy_in_one(smem0 + s * stage_bytes, pw, kI8TileBytes, full(s));
@@ -633,6 +635,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
             px += step_x;
         };
         if (!kTokens) wait_previous_launch();
+        allow_next_launch(); // (TMEM has been taken)
         for (int s = 0; s < early; s++) copy_x(s);
         int s = 0, phase = 0, filled = early;
         for (; filled < nk; filled++) {
@@ -647,6 +650,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
         for (int j = filled < a.stages ? 0 : filled - a.stages; j < filled; j++) mbar_wait_warp(full(j % a.stages), (j / a.stages) & 1);
     } else if (warp == 1) {
         // ---- products: lanes are output columns, columns of TMEM output rows
+        if (!kTokens) wait_previous_launch(); // (which may take longer than a bounded wait)
         const uint32_t idesc = product_idesc(128, a.rows, a.p.b.mn_major, a.p.a.mn_major);
         const uint32_t adv_w = a.p.b.mn_major ? 4096 >> 4 : 32 >> 4, adv_x = a.p.a.mn_major ? 4096 >> 4 : 32 >> 4;
         const uint64_t desc_w = tile_desc(smem0), desc_x = tile_desc(kTokens ? tokens0 : smem0 + kI8TileBytes);
@@ -923,7 +927,7 @@ int launch_i8_tokens(const void *x, int dtype, long long stride, const I8Product
     a.whole_rows = p.m * p.k * (long long)dtype_bytes(dtype) <= 16 * 1024;
     a.x_vec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(stride * (long long)dtype_bytes(dtype))) & 15) == 0;
 #define REXSC_I8_TOKENS(X)                                                                                             \
-    launch_cluster<product_split_kernel<X>, kSplitSmemMost>(a, tiles *a.split, a.split, kSplitThreads, smem, false, st, \
+    launch_cluster<product_split_kernel<X>, kSplitSmemMost>(a, tiles *a.split, a.split, kSplitThreads, smem, true, st,  \
                                                             "product_split_kernel")
     return dtype == REXSC_F32 ? REXSC_I8_TOKENS(float) : dtype == REXSC_F16 ? REXSC_I8_TOKENS(__half) : REXSC_I8_TOKENS(__nv_bfloat16);
 #undef REXSC_I8_TOKENS

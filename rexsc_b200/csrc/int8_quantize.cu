@@ -19,7 +19,8 @@ __global__ void __launch_bounds__(kQThreads, sizeof(T) == 4 ? 3 : 4)
 quantize_rows_kernel(const T *__restrict__ x, long long rows, long long cols, long long stride, int vec, long long rows_out,
                      long long tcols, int8_t *__restrict__ data, float *__restrict__ scale)
 {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_previous_launch();
+    allow_next_launch();
     __shared__ uint32_t part[2][8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int team = warp / kWarps, sub = threadIdx.x - team * 32 * kWarps; // row of the block, place among its threads
@@ -87,15 +88,14 @@ int quantize_rows(const T *x, long long rows, long long cols, long long stride, 
     const int vec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(stride * (long long)sizeof(T))) & 15) == 0;
     auto launch = [&](auto kernel, int rows_per_block) {
         const long long blocks = (rows_out + rows_per_block - 1) / rows_per_block, most = 148 * (sizeof(T) == 4 ? 3 : 4);
-        kernel<<<(unsigned)(blocks < most ? blocks : most), kQThreads, 0, st>>>(x, rows, cols, stride, vec, rows_out, tcols, data, scale);
+        return launch_under("quantize_rows_kernel", kernel, (unsigned)(blocks < most ? blocks : most), kQThreads, 0, st, x, rows,
+                            cols, stride, vec, rows_out, tcols, data, scale);
     };
     // as many warps as leave every lane at most kChunks chunks, where eight can
-    if (cols <= 32 * 8 * kChunks) launch(quantize_rows_kernel<T, 1>, 8);
-    else if (cols <= 64 * 8 * kChunks) launch(quantize_rows_kernel<T, 2>, 4);
-    else if (cols <= 128 * 8 * kChunks) launch(quantize_rows_kernel<T, 4>, 2);
-    else launch(quantize_rows_kernel<T, 8>, 1);
-    REXSC_LAUNCH_CHECK("quantize_rows_kernel");
-    return REXSC_OK;
+    if (cols <= 32 * 8 * kChunks) return launch(quantize_rows_kernel<T, 1>, 8);
+    if (cols <= 64 * 8 * kChunks) return launch(quantize_rows_kernel<T, 2>, 4);
+    if (cols <= 128 * 8 * kChunks) return launch(quantize_rows_kernel<T, 4>, 2);
+    return launch(quantize_rows_kernel<T, 8>, 1);
 }
 
 // plain row-major int8 <-> tiled
@@ -157,6 +157,8 @@ grad_amax_kernel(const T *__restrict__ dy, long long m, long long n, long long s
                  int rows, const float *__restrict__ row_scale, const float *__restrict__ col_scale,
                  uint32_t *__restrict__ row_most, uint32_t *__restrict__ col_most, float *__restrict__ sums)
 {
+    wait_previous_launch();
+    allow_next_launch();
     __shared__ float cmax[8][kGCols], csum[8][kGCols];
     extern __shared__ uint32_t rmax[]; // [rows]; a row is always the same warp's
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -233,7 +235,8 @@ grad_quantize_kernel(const T *__restrict__ dy, long long m, long long n, long lo
                      const float *__restrict__ sums, int col_parts, long long tcols, int8_t *__restrict__ qg,
                      float *__restrict__ sg, int8_t *__restrict__ qh, float *__restrict__ sh, B *__restrict__ db)
 {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    wait_previous_launch();
+    allow_next_launch();
     __shared__ float row_a[kI8Tile], row_inv[kI8Tile], row_s[kI8Tile];
     __shared__ __align__(16) float col_a[kGCols], col_inv[kGCols], col_s[kGCols];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -414,21 +417,20 @@ int grad_quantize(const T *dy, long long m, long long n, long long stride, const
     const long long tcols = i8_tiles(n), col_blocks = (n + kGCols - 1) / kGCols, blocks = col_blocks * i8_tiles(m);
     const size_t smem = (size_t)g.rows * 4;
     if (blocks > 0x7fffffffll) return REXSC_E_UNSUPPORTED;
-    grad_amax_kernel<T><<<(unsigned)(g.col_blocks * g.row_blocks), 256, smem, st>>>(
-        dy, m, n, stride, vec, (unsigned)g.col_blocks, g.tiles, g.rows, want_dw ? row_scale : nullptr,
-        want_dx ? col_scale : nullptr, want_dx ? b.row_most : nullptr, want_dw ? b.col_most : nullptr, db ? b.sums : nullptr);
-    REXSC_LAUNCH_CHECK("grad_amax_kernel");
-#define REXSC_I8_GRAD(B)                                                                                               \
-    grad_quantize_kernel<T, B><<<(unsigned)blocks, 256, 0, st>>>(                                                     \
-        dy, m, n, stride, vec, (unsigned)col_blocks, row_scale, col_scale, b.row_most, g.col_blocks, b.col_most,      \
-        b.sums, g.row_blocks, tcols, want_dx ? b.qg : nullptr, b.sg, want_dw ? b.qh : nullptr, b.sh,                  \
-        static_cast<B *>(db))
-    if (db_dtype == REXSC_F16) REXSC_I8_GRAD(__half);
-    else if (db_dtype == REXSC_BF16) REXSC_I8_GRAD(__nv_bfloat16);
-    else REXSC_I8_GRAD(float);
-#undef REXSC_I8_GRAD
-    REXSC_LAUNCH_CHECK("grad_quantize_kernel");
-    return REXSC_OK;
+    const int rc = launch_under("grad_amax_kernel", grad_amax_kernel<T>, (unsigned)(g.col_blocks * g.row_blocks), 256, smem, st,
+                                dy, m, n, stride, vec, (unsigned)g.col_blocks, g.tiles, g.rows, want_dw ? row_scale : nullptr,
+                                want_dx ? col_scale : nullptr, want_dx ? b.row_most : nullptr, want_dw ? b.col_most : nullptr,
+                                db ? b.sums : nullptr);
+    if (rc != REXSC_OK) return rc;
+    auto second = [&](auto *to) {
+        return launch_under("grad_quantize_kernel", grad_quantize_kernel<T, std::remove_pointer_t<decltype(to)>>, (unsigned)blocks,
+                            256, 0, st, dy, m, n, stride, vec, (unsigned)col_blocks, row_scale, col_scale, b.row_most,
+                            g.col_blocks, b.col_most, b.sums, g.row_blocks, tcols, want_dx ? b.qg : nullptr, b.sg,
+                            want_dw ? b.qh : nullptr, b.sh, to);
+    };
+    if (db_dtype == REXSC_F16) return second(static_cast<__half *>(db));
+    if (db_dtype == REXSC_BF16) return second(static_cast<__nv_bfloat16 *>(db));
+    return second(static_cast<float *>(db));
 }
 
 // operand whose contraction runs along the matrix's columns / rows

@@ -472,6 +472,95 @@ def test_captured_forward_and_backward(ops):
                 assert torch.equal(a, b)
 
 
+# ---- order of launches that begin under the end of the one before them --------------------------------------------
+@pytest.mark.parametrize("m", [1, 8, 64, 600])
+@pytest.mark.parametrize("kernel", ["auto", "split", "pair"])
+def test_calls_behind_one_another(ops, m, kernel):
+    """Weights quantised right before they are used, in memory that the call before still reads; tokens written right before
+    by another kernel: the same as call by call."""
+    n, k = 700, 1300
+    xs, ws = [_rand((m, k), BF16, seed=i) for i in range(3)], [_rand((n, k), BF16, seed=10 + i, scale=0.1) for i in range(4)]
+    ops.set_int8_kernel(kernel)
+    try:
+        want = {}
+        for i in range(12):
+            x = xs[i % 3] * 2
+            torch.cuda.synchronize()
+            w = ops.int8_quantize(ws[i % 4])
+            torch.cuda.synchronize()
+            want[i] = ops.int8_linear(x, w)
+            torch.cuda.synchronize()
+            del w
+        got = []
+        for i in range(120):
+            x = xs[i % 3] * 2
+            w = ops.int8_quantize(ws[i % 4])
+            got.append(ops.int8_linear(x, w))
+            del w, x
+    finally:
+        ops.set_int8_kernel("auto")
+    assert all(torch.equal(y, want[i % 12]) for i, y in enumerate(got))
+    assert ops.int8_status() == 0
+
+
+@pytest.mark.parametrize("m, n, k", [(40, 256, 300), (600, 700, 500), (2000, 16, 2900)])
+def test_training_steps_behind_one_another(ops, m, n, k):
+    """Forward, backward and the step that changes the weights, without a pause and step by step."""
+    from rexsc_b200 import optim
+
+    xs, dys = [_rand((m, k), BF16, seed=i) for i in range(3)], [_rand((m, n), BF16, seed=5 + i) for i in range(3)]
+
+    def train(pause):
+        w, b = torch.nn.Parameter(_rand((n, k), F32, seed=9, scale=0.05)), torch.nn.Parameter(_rand((n,), seed=8))
+        opt, out = optim.AdamW([w, b], lr=1e-2, state_bits=8), []
+        for i in range(20):
+            x = xs[i % 3].clone().requires_grad_()
+            y = ops.int8_linear(x, w, b)
+            pause()
+            y.backward(dys[i % 3])
+            pause()
+            opt.step()
+            pause()
+            out += [y.detach(), x.grad, w.grad, b.grad]
+            opt.zero_grad()
+        return out + [w.detach(), b.detach()]
+
+    for a, b in zip(train(lambda: None), train(torch.cuda.synchronize)):
+        assert torch.equal(a, b)
+    assert ops.int8_status() == 0
+
+
+@pytest.mark.parametrize("before", ["nothing", "copy", "fill", "join"])
+@pytest.mark.parametrize("m", [1, 64, 600])
+def test_captured_behind_anything(ops, m, before):
+    """What a call follows in a captured graph need not be a kernel."""
+    x, w = _rand((m, 1300), BF16), ops.int8_quantize(_rand((700, 1300), BF16, seed=1))
+    want, zero = ops.int8_linear(x, w), ops.int8_linear(torch.zeros_like(x), w)
+    into, other = torch.zeros_like(x), torch.cuda.Stream()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    ops.int8_linear(into, w)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        if before == "copy":
+            into.copy_(x)
+        elif before == "fill":
+            into.zero_()
+        elif before == "join":
+            other.wait_stream(stream)
+            with torch.cuda.stream(other):
+                into.copy_(x)
+            into2 = into.new_ones(5) * 2
+            stream.wait_stream(other)
+        y = ops.int8_linear(into, w)
+        z = ops.int8_linear(into, w)
+    for fill in (x, torch.zeros_like(x)):
+        into.copy_(fill)
+        graph.replay()
+        torch.cuda.synchronize()
+        expect = want if before in ("copy", "join") or (before == "nothing" and fill is x) else zero
+        assert torch.equal(y, expect) and torch.equal(z, expect)
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------------
 def test_refusals(ops):
     x, w = _rand((4, 64)), _rand((8, 64))
