@@ -325,7 +325,9 @@ int rexsc_fxp_conv2d_fwd(const rexsc_fxp_conv_desc *desc, const void *d_act, con
  * with d_w null, d_wq and d_w_scale are read instead (weights that are not trained).
  * `kernel`: REXSC_INT8_AUTO, or one of the two product kernels; results are identical.
  * rexsc_int8_status synchronises the stream and returns REXSC_E_DEVICE_TIMEOUT if a bounded device-side wait of an int8
- * product on the current device gave up since it was last asked (that call's outputs are incomplete), else REXSC_OK.
+ * product on the current device gave up since it was last asked (that call's outputs are incomplete: what was not computed is
+ * not written), else REXSC_OK.  rexsc_int8_test_waits, for tests of that: in the product launches that follow in this process
+ * the waits of all blocks (-2), of none (-1) or, in the kernel of REXSC_INT8_SPLIT, of the given block give up at once.
  */
 #define REXSC_INT8_MAX_DOT 131071
 enum { REXSC_INT8_AUTO = 0, REXSC_INT8_SPLIT = 1, REXSC_INT8_PAIR = 2 };
@@ -351,6 +353,7 @@ int rexsc_int8_linear_bwd(const void *d_dy, int32_t dtype, int64_t m, int64_t n,
                           int32_t dx_dtype, void *d_dw, int32_t dw_dtype, void *d_db, int32_t db_dtype, int32_t kernel,
                           void *d_workspace, size_t workspace_bytes, void *stream);
 int rexsc_int8_status(void *stream);
+int rexsc_int8_test_waits(int64_t block);
 
 /*
  * One AdamW step over many tensors.  The reference's loops take torch's optimizers (main_imagenet.py:212-213,

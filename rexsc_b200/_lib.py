@@ -93,6 +93,7 @@ SYMBOLS = {
     "rexsc_int8_linear_bwd": (C.c_int, [_vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp,
                                         _i32, _i32, _vp, _sz, _vp]),
     "rexsc_int8_status": (C.c_int, [_vp]),
+    "rexsc_int8_test_waits": (C.c_int, [_i64]),
     "rexsc_adamw_step": (C.c_int, [C.POINTER(AdamWDesc), _vp, _i32, _vp]),
     "rexsc_alu_probe": (C.c_int, [_i32, _i32, _vp, _vp]),
     "rexsc_mma_probe": (C.c_int, [_i32, _i32, _i32, _vp, _vp]),

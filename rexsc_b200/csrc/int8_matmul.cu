@@ -14,7 +14,8 @@
 //                        to 32 tokens as they are, which it quantises itself.  Bound by latencies in a row: one token
 //                        through 4096 x 4096 in 7.8 us, of which the weights' 17 MB take 2.6.
 // Every mbarrier wait is bounded; a CTA whose wait gives up raises the library's status word (rexsc_int8_status), stores
-// nothing more, waits for its copies in flight, frees its TMEM and leaves.
+// nothing more (nor does any CTA that would have joined its sums), waits, again with a limit, for its copies and products in
+// flight, frees its TMEM and leaves.
 #include <atomic>
 #include <cuda.h>
 
@@ -27,6 +28,15 @@ namespace {
 __device__ int g_i8_status = 0; // != 0: a bounded wait gave up since rexsc_int8_status was last asked
 
 constexpr uint32_t kWaitLimit = 1u << 22;
+// The block whose waits give up without asking, so that tests see what a call does then; waits for what is in flight keep
+// their limit.  In the split kernel no CTA waits for another one's copies or products, so it can be any block; in the pair
+// kernel they do, so that there it is all blocks or none.
+constexpr unsigned kNobody = ~0u, kEverybody = ~0u - 1;
+std::atomic<unsigned> g_hasty{kNobody};
+__device__ __forceinline__ uint32_t wait_limit(unsigned hasty)
+{
+    return hasty == kEverybody || hasty == blockIdx.x ? 0u : kWaitLimit;
+}
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -34,9 +44,9 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
 {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity)
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t limit = kWaitLimit)
 {
-    for (uint32_t i = 0; i < kWaitLimit; i++) {
+    for (uint32_t i = 0; i < limit; i++) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -49,9 +59,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity)
     return false;
 }
 // by a whole warp, with one answer
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity)
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, uint32_t limit = kWaitLimit)
 {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit));
 }
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes)
 {
@@ -209,6 +219,7 @@ struct PairArgs {
     long long tiles_i, tiles_j; // 256 x 256 output tiles
     int k_blocks;
     int store_bytes;            // bytes that every row of the output is aligned to: 32, 16, or fewer
+    unsigned hasty;
 };
 
 constexpr int kPairStages = 6;
@@ -281,6 +292,7 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
     const int warp = warp_number(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const long long first = blockIdx.x >> 1, step = gridDim.x >> 1, tiles = a.tiles_i * a.tiles_j;
+    const uint32_t limit = wait_limit(a.hasty);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kPairStages; s++) {
@@ -329,7 +341,7 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
                 int row_a = (int)(ia * a.p.a.step_mn) * kI8Tile, row_b = (int)(ib * a.p.b.step_mn) * kI8Tile;
                 for (int k = a.k_blocks; k > 0; k--) {
                     if (filled == kPairStages) {
-                        if (!(ok = mbar_wait(empty(r.at), r.phase ^ 1))) break;
+                        if (!(ok = mbar_wait(empty(r.at), r.phase ^ 1, limit))) break;
                     } else {
                         filled++;
                     }
@@ -357,10 +369,10 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
             bool ok = true;
             for (long long t = first; t < tiles && ok; t += step, turn++) {
                 const int b = turn & 1;
-                if (turn >= 2 && !(ok = mbar_wait_warp(acc_empty(b), (turn / 2 - 1) & 1))) break;
+                if (turn >= 2 && !(ok = mbar_wait_warp(acc_empty(b), (turn / 2 - 1) & 1, limit))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (int k = 0; k < a.k_blocks; k++) {
-                    if (!(ok = mbar_wait_warp(full(r.at), r.phase))) break;
+                    if (!(ok = mbar_wait_warp(full(r.at), r.phase, limit))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t da = desc0 + r.at * (kPairStageBytes >> 4);
                     product_step<2>(tmem + b * 256, da, da + (kI8TileBytes >> 4), adv_a, adv_b, idesc, k > 0);
@@ -393,7 +405,7 @@ product_pair_kernel(const __grid_constant__ PairArgs a)
             const float rs = row < a.p.m ? a.p.row_scale[row] : 0.f;
             asm volatile("bar.sync 1, 128;" ::: "memory");
             // one lane of a warp asks: 128 threads that poll cost the copying thread a fifth of its rate
-            const bool there = lane != 0 || mbar_wait(acc_full(b), (turn / 2) & 1);
+            const bool there = lane != 0 || mbar_wait(acc_full(b), (turn / 2) & 1, limit);
             if (!__all_sync(0xffffffffu, there)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -458,6 +470,7 @@ struct SplitArgs {
     long long x_stride;
     int x_vec;          // its rows begin on 16 bytes
     int whole_rows;     // every CTA reads whole rows for their largest magnitudes
+    unsigned hasty;
 };
 
 constexpr int kSplitThreads = 128;
@@ -500,7 +513,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
     constexpr bool kTokens = !std::is_same<X, int8_t>::value;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * kSplitMaxStages + 1];
-    __shared__ uint32_t tmem_slot;
+    __shared__ uint32_t tmem_slot, gave_up; // gave_up: 1 once a wait of this CTA has given up
     __shared__ uint32_t part_most[kTokenRows];
     __shared__ float row_a[kTokenRows], row_inv[kTokenRows], row_s[kSplitThreads];
     uint8_t *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -520,6 +533,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
     const uint32_t smem0 = smem_addr(smem), stage_bytes = kI8TileBytes + (kTokens ? 0 : a.q_bytes);
     const uint32_t tokens0 = smem0 + a.stages * stage_bytes; // the quantised tokens, [128 columns][rows][128 bytes]
     const int early = nk < a.stages ? nk : a.stages;
+    const uint32_t limit = wait_limit(args.hasty);
 
     if (kTokens) wait_previous_launch(); // (it may be the one that quantises the weights)
     const int8_t *pw = a.p.b.data + ((size_t)(tj * a.p.b.step_mn) + (size_t)(k0 * a.p.b.step_k)) * kI8TileBytes;
@@ -528,6 +542,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
         if (lane == 0) {
             for (int s = 0; s < a.stages; s++) mbar_init(full(s), 1), mbar_init(empty(s), 1);
             mbar_init(acc_full, 1);
+            gave_up = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
@@ -639,7 +654,7 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
         for (int s = 0; s < early; s++) copy_x(s);
         int s = 0, phase = 0, filled = early;
         for (; filled < nk; filled++) {
-            if (!mbar_wait_warp(empty(s), phase)) break;
+            if (!mbar_wait_warp(empty(s), phase, limit)) break; // (the products' warp then gives up too)
             mbar_expect_one(full(s), stage_bytes);
             copy_in_one(smem0 + s * stage_bytes, pw, kI8TileBytes, full(s));
             pw += step_w;
@@ -656,7 +671,10 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
         const uint64_t desc_w = tile_desc(smem0), desc_x = tile_desc(kTokens ? tokens0 : smem0 + kI8TileBytes);
         int s = 0, phase = 0;
         for (int i = 0; i < nk; i++) {
-            if (!mbar_wait_warp(full(s), phase)) break;
+            if (!mbar_wait_warp(full(s), phase, limit)) {
+                gave_up = 1;
+                break;
+            }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             product_step<1>(tmem, desc_w + (s * stage_bytes >> 4), desc_x + ((kTokens ? i * a.q_bytes : s * stage_bytes) >> 4),
                             adv_w, adv_x, idesc, i > 0);
@@ -671,8 +689,15 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
         if (threadIdx.x < rows) row_s[threadIdx.x] = a.p.row_scale[row0 + threadIdx.x];
         __syncwarp();
     }
-    if (lane == 0) mbar_wait(acc_full, 0); // (one lane of a warp asks)
-    __syncwarp();
+    bool done = true;
+    if (lane == 0) { // (one lane of a warp asks)
+        done = mbar_wait(acc_full, 0, limit);
+        if (!done) { // products in flight read this CTA's stages and write its TMEM
+            gave_up = 1;
+            mbar_wait(acc_full, 0);
+        }
+    }
+    done = __all_sync(0xffffffffu, done);
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_lane = tmem + ((uint32_t)(warp * 32) << 16);
     auto free_tmem = [&]() {
@@ -683,9 +708,10 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)a.tmem_cols) : "memory");
         }
     };
-    // sums to shared memory, [row][column]; every CTA of the cluster finishes some of the rows, four columns a lane
+    // sums to shared memory, [row][column]; every CTA of the cluster finishes some of the rows, four columns a lane.  (The copies
+    // have landed where the sums go: all of them have been multiplied, or a wait gave up and the sums are not used.)
     int *red = reinterpret_cast<int *>(smem);
-    for (int c = 0; c < rows; c += 16) {
+    for (int c = 0; c < rows && done; c += 16) {
         int v[16];
         __syncwarp();
         tmem_load16(tmem_lane + c, v);
@@ -699,29 +725,34 @@ product_split_kernel(const __grid_constant__ SplitArgs args)
     __syncwarp();
     if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     const long long col = col0 + lane * 4;
-    const int live = a.p.n - col < 4 ? (int)(a.p.n - col) : 4;
-    if (live > 0) {
-        float cs[4], bias[4];
+    const int live = a.p.n - col < 4 ? (int)(a.p.n - col) : 4; // (0 or less behind the last column: nothing is stored)
+    float cs[4], bias[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            cs[i] = i < live && a.p.col_scale ? a.p.col_scale[col + i] : 1.f;
-            bias[i] = i < live && a.p.bias ? load_any(a.p.bias, a.p.bias_dtype, col + i) : 0.f;
+    for (int i = 0; i < 4; i++) {
+        cs[i] = i < live && a.p.col_scale ? a.p.col_scale[col + i] : 1.f;
+        bias[i] = i < live && a.p.bias ? load_any(a.p.bias, a.p.bias_dtype, col + i) : 0.f;
+    }
+    // whether any CTA of the cluster gave up: a lane asks one of them (the answer travels beside the first sums)
+    uint32_t bad;
+    if (split > 1)
+        asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(bad) : "r"(map_rank(smem_addr(&gave_up), lane & (split - 1))) : "memory");
+    else
+        bad = gave_up;
+    for (int c = rank * 4 + warp; c < rows; c += 4 * split) {
+        int4 sum = *reinterpret_cast<const int4 *>(red + c * 128 + lane * 4);
+        const uint32_t at = smem_addr(red + c * 128 + lane * 4);
+        for (int i = 1; i < split; i++) {
+            const int r = (rank + i) & (split - 1); // (each starts with another one)
+            int4 v;
+            asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(map_rank(at, r)) : "memory");
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
         }
-        for (int c = rank * 4 + warp; c < rows; c += 4 * split) {
-            int4 sum = *reinterpret_cast<const int4 *>(red + c * 128 + lane * 4);
-            const uint32_t at = smem_addr(red + c * 128 + lane * 4);
-            for (int i = 1; i < split; i++) {
-                const int r = (rank + i) & (split - 1); // (each starts with another one)
-                int4 v;
-                asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(map_rank(at, r)) : "memory");
-                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-            }
-            const float rs = row_s[c];
-            const float f[4] = {scaled(sum.x, rs, cs[0], bias[0]), scaled(sum.y, rs, cs[1], bias[1]),
-                                scaled(sum.z, rs, cs[2], bias[2]), scaled(sum.w, rs, cs[3], bias[3])};
-            store4(a.p.out, a.p.out_dtype, (row0 + c) * a.p.out_stride + col, f, live, a.store_bytes >= 16);
-        }
+        const float rs = row_s[c];
+        const float f[4] = {scaled(sum.x, rs, cs[0], bias[0]), scaled(sum.y, rs, cs[1], bias[1]),
+                            scaled(sum.z, rs, cs[2], bias[2]), scaled(sum.w, rs, cs[3], bias[3])};
+        if (__any_sync(0xffffffffu, bad)) break;
+        store4(a.p.out, a.p.out_dtype, (row0 + c) * a.p.out_stride + col, f, live, a.store_bytes >= 16);
     }
     if (split > 1) cluster_sync(); // the others still read this CTA's sums
 }
@@ -814,6 +845,7 @@ int launch_pair(const I8Product &p, bool overlap, cudaStream_t st)
     a.tiles_j = (p.n + 255) / 256;
     a.k_blocks = (int)i8_tiles(p.k);
     a.store_bytes = store_alignment(p);
+    a.hasty = g_hasty.load(std::memory_order_relaxed) == kEverybody ? kEverybody : kNobody;
     const long long tiles = a.tiles_i * a.tiles_j, pairs = tiles < 74 ? tiles : 74;
     return launch_cluster<product_pair_kernel<T>, kPairSmem>(a, pairs * 2, 0, kPairThreads, kPairSmem, overlap, st, "product_pair_kernel");
 }
@@ -871,6 +903,7 @@ size_t split_stages(SplitProblem *a, int split, bool tokens)
 int launch_split(const I8Product &p, const I8Product *second, bool overlap, cudaStream_t st)
 {
     SplitArgs a = {};
+    a.hasty = g_hasty.load(std::memory_order_relaxed);
     const long long tiles = split_shape(&a.p[0], p), more = second ? split_shape(&a.p[1], *second) : 0;
     int k_blocks = a.p[0].k_blocks;
     if (second && a.p[1].k_blocks < k_blocks) k_blocks = a.p[1].k_blocks;
@@ -916,6 +949,7 @@ bool i8_tokens_fit(long long m, long long n, long long k, int kernel)
 int launch_i8_tokens(const void *x, int dtype, long long stride, const I8Product &p, cudaStream_t st)
 {
     SplitArgs a = {};
+    a.hasty = g_hasty.load(std::memory_order_relaxed);
     const long long tiles = split_shape(&a.p[0], p);
     a.split = split_of(tiles, a.p[0].k_blocks);
     const size_t smem = split_stages(&a.p[0], a.split, true);
@@ -945,4 +979,12 @@ extern "C" int rexsc_int8_status(void *stream)
     REXSC_CUDA_CHECK(cudaStreamSynchronize(st));
     if (seen) REXSC_CUDA_CHECK(cudaMemcpyToSymbolAsync(g_i8_status, &none, sizeof(none), 0, cudaMemcpyHostToDevice, st));
     return seen ? REXSC_E_DEVICE_TIMEOUT : REXSC_OK;
+}
+
+extern "C" int rexsc_int8_test_waits(int64_t block)
+{
+    using namespace rexsc;
+    if (block < -2 || block > 0x7fffffffll) return REXSC_E_BAD_ARG;
+    g_hasty.store(block == -1 ? kNobody : block == -2 ? kEverybody : (unsigned)block, std::memory_order_relaxed);
+    return REXSC_OK;
 }
