@@ -99,7 +99,8 @@ struct Int8Linear : public torch::autograd::Function<Int8Linear> {
         const bool want_b = bias.defined() && bias.requires_grad();
         const Tensor x2 = rows_of(x, k);
         const int64_t m = x2.size(0), code = code_of(x2.scalar_type());
-        Tensor y = at::empty({m, n}, x2.options());
+        // (made in its final shape: a view made here could not be written to in place)
+        Tensor y = at::empty(with_last(x, n), x2.options());
         Tensor buf;
         int64_t at_w = 0;
         if (m > 0) {
@@ -128,7 +129,7 @@ struct Int8Linear : public torch::autograd::Function<Int8Linear> {
                                                         (int64_t)(weight.defined() ? weight.scalar_type() : at::kFloat),
                                                         (int64_t)(bias.defined() ? bias.scalar_type() : at::kFloat)};
         ctx->saved_data["shape"] = x.sizes().vec();
-        return x.dim() == 2 ? y : y.view(with_last(x, n));
+        return y;
     }
 
     static variable_list backward(AutogradContext *ctx, variable_list grads)
@@ -157,7 +158,7 @@ struct Int8Linear : public torch::autograd::Function<Int8Linear> {
                 const float *ws = reinterpret_cast<const float *>(wq + tile_bytes(n, k));
                 if (saved[1].defined()) wq = static_cast<const int8_t *>(saved[1].data_ptr()), ws = saved[2].data_ptr<float>();
                 const Tensor g = rows_of(dy, n);
-                if (want_x) dx = at::empty({m, k}, options(xt));
+                if (want_x) dx = at::empty(shape, options(xt));
                 if (want_w) dw = at::empty({n, k}, options(wt));
                 if (want_b) db = at::empty({n}, options(bt));
                 const auto ptr = [](const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
@@ -169,7 +170,6 @@ struct Int8Linear : public torch::autograd::Function<Int8Linear> {
                                             ptr(dw), code(dw), ptr(db), code(db), (int)kernel, scratch.data_ptr(), nbytes,
                                             stream_of(dev)),
                       "rexsc_int8_linear_bwd");
-                if (want_x && shape.size() != 2) dx = dx.view(shape);
             }
             if (want_x && dx.scalar_type() != xt) dx = dx.to(xt);
             if (want_w && dw.scalar_type() != wt) dw = dw.to(wt);
@@ -229,7 +229,7 @@ Tensor int8_linear(const Tensor &x, const std::optional<Tensor> &weight_, const 
     const int64_t m = x2.size(0);
     const int code = code_of(x2.scalar_type());
     const Bias b(bias, n, dev);
-    Tensor y = at::empty({m, n}, x2.options());
+    Tensor y = at::empty(with_last(x, n), x2.options());
     if (m > 0) {
         void *const st = stream_of(dev);
         Tensor kept;
@@ -251,7 +251,7 @@ Tensor int8_linear(const Tensor &x, const std::optional<Tensor> &weight_, const 
                                     (int)kernel, nbytes ? scratch.data_ptr() : nullptr, nbytes, st),
               "rexsc_int8_linear_fwd");
     }
-    return x.dim() == 2 ? y : y.view(with_last(x, n));
+    return y;
 }
 
 // ---- AdamW ----------------------------------------------------------------------------------------------------------
