@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/rexsc_b200.h"
@@ -189,6 +190,8 @@ struct Int8Linear : public torch::autograd::Function<Int8Linear> {
     }
 };
 
+bool has_tangent(const Tensor &t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+
 // weight: floating point [n, k], or undefined with data and scale of weights quantised before
 Tensor int8_linear(const Tensor &x, const std::optional<Tensor> &weight_, const std::optional<Tensor> &data_,
                    const std::optional<Tensor> &scale_, int64_t n, int64_t k, const std::optional<Tensor> &bias_, int64_t kernel)
@@ -196,6 +199,11 @@ Tensor int8_linear(const Tensor &x, const std::optional<Tensor> &weight_, const 
     const Tensor weight = weight_.value_or(Tensor()), data = data_.value_or(Tensor()), scale = scale_.value_or(Tensor());
     const Tensor bias = bias_.value_or(Tensor());
     const bool prepared = data.defined();
+    // a trace would record the output's allocation and not the launches; a tangent would be lost, which reads as a slope of 0
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), "int8_linear cannot be traced");
+    TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() ||
+                                    !(has_tangent(x) || has_tangent(weight) || has_tangent(bias)),
+                                "int8_linear has no forward-mode derivative");
     TORCH_CHECK(x.is_cuda(), "int8_linear: expected a CUDA tensor (rexsc_b200 has no CPU path)");
     if (!prepared) {
         TORCH_CHECK(weight.is_cuda(), "int8_linear: expected a CUDA tensor (rexsc_b200 has no CPU path)");

@@ -684,6 +684,11 @@ def _int8_kernel() -> int:
     return getattr(_kernel_choice, "int8", _lib.INT8_AUTO)
 
 
+def _not_traced(what: str) -> None:
+    if torch._C._is_tracing():  # a trace would record the allocations and not the launches
+        raise NotImplementedError(f"{what} cannot be traced")
+
+
 class Int8Matrix:
     """A matrix in 8-bit integers with an fp32 scale per row, as :func:`int8_quantize` makes it: row r stands for
     ``values()[r] * scale[r]``.  ``data`` holds the integers in the library's own layout; keep the object as the prepared
@@ -726,6 +731,7 @@ class Int8Matrix:
     @classmethod
     def from_values(cls, values: torch.Tensor, scale: torch.Tensor) -> "Int8Matrix":
         """From int8 ``values`` [rows, cols] and their ``scale`` [rows]."""
+        _not_traced("Int8Matrix.from_values")
         _require_cuda(values, "Int8Matrix.from_values")
         if values.dtype != torch.int8 or values.dim() != 2 or 0 in values.shape:
             raise ValueError("Int8Matrix.from_values: expected int8 values [rows, cols], neither of them 0")
@@ -742,6 +748,7 @@ class Int8Matrix:
 
     def values(self) -> torch.Tensor:
         """The integers, int8 [rows, cols]."""
+        _not_traced("Int8Matrix.values")
         self._check("Int8Matrix.values")
         dev = self.data.device
         with _on(dev):
@@ -785,6 +792,7 @@ def int8_quantize(x: torch.Tensor) -> Int8Matrix:
     """Rows of ``x`` [rows, cols] (tokens of activations, output channels of weights) in 8-bit integers: the scale of a row is
     ``max|x| / 127``, its integers are the exact quotients rounded to the nearest, ties to even.  A row of zeros has the scale
     0; a row that holds an infinity or a NaN has the scale NaN and zeros, so that its products are NaN and no other row's."""
+    _not_traced("int8_quantize")
     _require_cuda(x, "int8_quantize")
     if x.dim() != 2 or 0 in x.shape or not x.is_floating_point():
         raise ValueError("int8_quantize: expected floating-point [rows, cols], neither of them 0")
@@ -816,8 +824,10 @@ def _int8_matmul(a: Int8Matrix, b: Int8Matrix, bias, dtype: torch.dtype, what: s
 @_traced
 def int8_matmul(a: Int8Matrix, b: Int8Matrix, bias: torch.Tensor = None, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``a b^T`` [a.rows, b.rows]: exact sums of the products of the integers, times both rows' scales, plus ``bias``
-    [b.rows], in fp32 and rounded once to ``dtype`` (float32, float16 or bfloat16)."""
+    [b.rows], in fp32 and rounded once to ``dtype`` (float32, float16 or bfloat16).  Like :func:`int8_quantize` it passes no
+    gradients on, to the bias neither: :func:`int8_linear` does."""
     what = "int8_matmul"
+    _not_traced(what)
     if not isinstance(a, Int8Matrix) or not isinstance(b, Int8Matrix):
         raise ValueError(f"{what}: expected two Int8Matrix operands")
     if a.cols != b.cols or a.device != b.device:
@@ -843,6 +853,8 @@ def int8_linear(x: torch.Tensor, weight, bias: torch.Tensor = None) -> torch.Ten
     which is then quantised per token for ``dx`` and per output channel for ``dw``; the bias's gradient is the plain sum.
 
     Sums are exact up to 131071 products: ``k``, and in training ``n`` (for ``dx``) and the number of tokens (for ``dw``).
+
+    There is no second and no forward-mode derivative, and a call cannot be traced: all three raise.
 
     Both directions can be captured into a CUDA graph; every call has scratch of its own.  As with any op of torch, drop all
     eager graphs of the same leaves (outputs that still hold one) before capturing a backward pass: torch's engine would wait
