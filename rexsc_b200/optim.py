@@ -193,10 +193,14 @@ class AdamW(torch.optim.Optimizer):
 
     # -- step ---------------------------------------------------------------------------------------------------
     def step(self, closure=None):
+        args, kwargs = (self,) if closure is None else (self, closure), {}
         for hook in (*_PRE_HOOKS.values(), *self._optimizer_step_pre_hooks.values()):
-            changed = hook(self, (self, closure), {})
+            changed = hook(self, args, kwargs)
             if changed is not None:
-                closure = changed[0][1]
+                if not isinstance(changed, tuple) or len(changed) != 2:
+                    raise RuntimeError(f"AdamW: a step's pre-hook must return None or (args, kwargs), not {changed}")
+                args, kwargs = changed
+                closure = _closure_of(*args, **kwargs)
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -208,12 +212,17 @@ class AdamW(torch.optim.Optimizer):
             plan["native"].step(group["params"], 0.0 if on_device else float(lr), lr if on_device else None, b1, b2,
                                 group["eps"], group["weight_decay"], scale, inf)
         for hook in (*self._optimizer_step_post_hooks.values(), *_POST_HOOKS.values()):
-            hook(self, (self, closure), {})
+            hook(self, args, kwargs)
         return loss
 
     # torch wraps an optimizer's step in a profiler range and calls the hooks there, 10 us of the host's time in a step
     # whose launch takes 4; the hooks are called above instead
     step.hooked = True
+
+
+def _closure_of(optimizer, closure=None):
+    """The closure among a step's arguments as a hook has left them."""
+    return closure
 
 
 def _dense(t: torch.Tensor) -> bool:
