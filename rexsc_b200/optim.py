@@ -6,6 +6,7 @@ place in ``utils_own.train``: it is a ``torch.optim.Optimizer``, so learning-rat
 """
 from __future__ import annotations
 
+import copy
 from typing import Dict
 
 import torch
@@ -169,6 +170,13 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict) -> None:
+        """Takes over copies of a state's moments and numbers, none of its tensors.  Where a group's ``lr`` is a tensor it stays
+        that tensor and gets the saved value, so that a captured step goes on reading the right one."""
+        state_dict = state_dict.copy()
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            if changed is not None:
+                state_dict = changed
         groups = state_dict["param_groups"]
         if state_dict.get("state_bits") != self._state_bits:
             raise ValueError(f"AdamW: the state was saved with state_bits={state_dict.get('state_bits')}, not {self._state_bits}")
@@ -189,7 +197,13 @@ class AdamW(torch.optim.Optimizer):
         for mine, theirs in todo:
             mine.copy_(theirs)
         for group, saved in zip(self.param_groups, groups):
-            group.update({k: v for k, v in saved.items() if k not in ("params", "strides")})
+            lr = group["lr"]
+            group.update({k: copy.deepcopy(v) for k, v in saved.items() if k not in ("params", "param_names", "strides")})
+            if isinstance(lr, torch.Tensor):
+                lr.fill_(group["lr"])
+                group["lr"] = lr
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     # -- step ---------------------------------------------------------------------------------------------------
     def step(self, closure=None):
