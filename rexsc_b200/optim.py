@@ -7,6 +7,7 @@ place in ``utils_own.train``: it is a ``torch.optim.Optimizer``, so learning-rat
 from __future__ import annotations
 
 import copy
+from collections.abc import Mapping
 from typing import Dict
 
 import torch
@@ -21,16 +22,52 @@ from . import _lib
 from .ops import _DTYPES, _on
 
 
-class _State(dict):
-    """Per-parameter views of the flat moment buffers, made when they are asked for."""
+class _Views(dict):
+    """A parameter's moments: views of the flat buffers.  What is assigned to one of them is copied into it."""
 
-    def __init__(self, make):
-        super().__init__()
-        self._make = make
+    def __setitem__(self, name, value):
+        if name not in self:
+            raise KeyError(f"AdamW: a parameter's state has {', '.join(self)}, and no {name}")
+        mine, value = self[name], torch.as_tensor(value)
+        if value.shape != mine.shape:
+            raise ValueError(f"AdamW: expected {name} {tuple(mine.shape)}, got {tuple(value.shape)}")
+        if value is not mine:
+            with torch.no_grad():
+                mine.copy_(value)
 
-    def __missing__(self, p):
-        self[p] = made = self._make(p)
+    def update(self, *args, **kwargs):
+        for name, value in dict(*args, **kwargs).items():
+            self[name] = value
+
+    def _refuse(self, *args, **kwargs):
+        raise TypeError("AdamW: a parameter's state cannot be taken away; zero_() its tensors")
+
+    __delitem__ = __ior__ = clear = pop = popitem = setdefault = _refuse
+
+
+class _State(Mapping):
+    """All parameters' views of the flat moment buffers, made when they are asked for."""
+
+    def __init__(self, place, make):
+        self._place, self._make, self._made = place, make, {}
+
+    def __getitem__(self, p) -> _Views:
+        made = self._made.get(p)
+        if made is None:
+            made = self._made[p] = _Views(self._make(p))
         return made
+
+    def __setitem__(self, p, value) -> None:
+        self[p].update(value)
+
+    def __contains__(self, p) -> bool:
+        return p in self._place
+
+    def __iter__(self):
+        return iter(self._place)
+
+    def __len__(self) -> int:
+        return len(self._place)
 
 
 BLOCK = 256  # elements of a block of the flat moment buffers (of a scale of 8-bit moments)
@@ -47,6 +84,9 @@ class AdamW(torch.optim.Optimizer):
     its mean over the steps is right (rounding to nearest would freeze them); it depends on the element's place and the step
     count alone, so runs repeat.  A gradient that is no finite number spoils its element, with 8 bits its block of 256.
 
+    ``state`` holds every parameter from the start on; its tensors are views of the buffers (:meth:`flat_state`), and what is
+    assigned to them is copied.
+
     ``lr`` may be a one-element float32 CUDA tensor, which a captured step then reads at every replay.  The number of steps
     is kept on the device, one count for each parameter group: weights without a gradient are left out of a step, but share
     their group's count.  16-bit weights are rounded to nearest at every step; there is no 32-bit copy of them."""
@@ -60,8 +100,19 @@ class AdamW(torch.optim.Optimizer):
         self._state_bits = state_bits
         self._plans = []
         self._place = {}    # parameter -> (its group's plan, its number there)
+        self._built = False
+        self._state = _State(self._place, self._views)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
-        self.state = _State(self._views)
+        self._built = True
+
+    @property
+    def state(self) -> _State:
+        return self._state
+
+    @state.setter
+    def state(self, value) -> None:
+        if self._built:  # (the base class begins with an empty one)
+            raise TypeError("AdamW: the state cannot be replaced: use load_state_dict(), or assign to its tensors")
 
     def __getstate__(self):
         raise TypeError("rexsc_b200.optim.AdamW cannot be copied or pickled: use state_dict()")
@@ -160,9 +211,8 @@ class AdamW(torch.optim.Optimizer):
     def state_dict(self):
         """As torch's optimizers give it; the tensors are the optimizer's own.  Moments in 8 bits are stored in the order of
         the weights' memory."""
-        for p in self._place:
-            self.state[p]
         sd = super().state_dict()
+        sd["state"] = {key: dict(views) for key, views in sd["state"].items()}
         sd["state_bits"] = self._state_bits
         for i, (strides, plan) in enumerate((p["strides"], p) for p in self._plans):
             sd["param_groups"][i]["strides"] = [tuple(s) for s in strides]
