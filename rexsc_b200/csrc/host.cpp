@@ -4,6 +4,7 @@
 // optimizer's plan.  (From Python over ctypes: one token through a 4096 x 4096 layer 12.3 us a call of which the GPU works 8.5,
 // a small training step 139 us, a step over 62 tensors 51 us.)
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -11,6 +12,9 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
+
+#include <cstdlib>
+#include <cstring>
 
 #include "../../include/rexsc_b200.h"
 
@@ -34,7 +38,8 @@ void check(int rc, const char *what)
                        : rc == REXSC_E_WORKSPACE   ? "REXSC_E_WORKSPACE"
                        : rc == REXSC_E_TOO_LONG    ? "REXSC_E_TOO_LONG"
                        : rc == REXSC_E_CUDA        ? "REXSC_E_CUDA"
-                                                   : "error";
+                       : rc == REXSC_E_DEVICE_TIMEOUT ? "REXSC_E_DEVICE_TIMEOUT"
+                                                      : "error";
     TORCH_CHECK_VALUE(rc != REXSC_E_BAD_ARG && rc != REXSC_E_UNSUPPORTED && rc != REXSC_E_TOO_LONG, what, ": ", name);
     TORCH_CHECK(false, what, ": ", name, rc == REXSC_E_CUDA ? ": " : "", rc == REXSC_E_CUDA ? rexsc_last_cuda_error() : "");
 }
@@ -57,6 +62,17 @@ Tensor rows_of(const Tensor &t, int64_t cols)
     Tensor r = code_of(t.scalar_type()) >= 0 ? t : t.to(at::kFloat);
     if (r.dim() != 2) r = r.reshape({-1, cols});
     return r.stride(1) == 1 || cols == 1 ? r : r.contiguous();
+}
+
+// With REXSC_B200_DEBUG=1, behind a product: whether a bounded wait gave up (the call synchronises; not during a capture)
+void check_waits(const at::Device &d, const char *what)
+{
+    static const bool debug = [] {
+        const char *v = std::getenv("REXSC_B200_DEBUG");
+        return v && std::strcmp(v, "1") == 0;
+    }();
+    if (debug && c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None)
+        check(rexsc_int8_status(stream_of(d)), what);
 }
 
 int64_t tile_bytes(int64_t rows, int64_t cols) { return (rows + 127) / 128 * ((cols + 127) / 128) * 16384; }
@@ -119,6 +135,7 @@ struct Int8Linear : public torch::autograd::Function<Int8Linear> {
                                               reinterpret_cast<float *>(base + tile_bytes(m, k)), wq, ws, y.data_ptr(), code,
                                               (int)kernel, stream_of(dev)),
                   "rexsc_int8_linear_train_fwd");
+            check_waits(dev, "int8_linear (device status)");
             if (weight.defined() && want_x && !want_w) { // the activations are not needed again: only the weights stay
                 buf = buf.slice(0, at_w).clone();
                 at_w = 0;
@@ -171,6 +188,7 @@ struct Int8Linear : public torch::autograd::Function<Int8Linear> {
                                             ptr(dw), code(dw), ptr(db), code(db), (int)kernel, scratch.data_ptr(), nbytes,
                                             stream_of(dev)),
                       "rexsc_int8_linear_bwd");
+                check_waits(dev, "int8_linear's gradients (device status)");
             }
             if (want_x && dx.scalar_type() != xt) dx = dx.to(xt);
             if (want_w && dw.scalar_type() != wt) dw = dw.to(wt);
@@ -258,6 +276,7 @@ Tensor int8_linear(const Tensor &x, const std::optional<Tensor> &weight_, const 
         check(rexsc_int8_linear_fwd(x2.data_ptr(), code, m, k, x2.stride(0), wq, ws, n, b.ptr, b.dtype, y.data_ptr(), code,
                                     (int)kernel, nbytes ? scratch.data_ptr() : nullptr, nbytes, st),
               "rexsc_int8_linear_fwd");
+        check_waits(dev, "int8_linear (device status)");
     }
     return y;
 }

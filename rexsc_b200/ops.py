@@ -817,6 +817,8 @@ def _int8_matmul(a: Int8Matrix, b: Int8Matrix, bias, dtype: torch.dtype, what: s
     _lib.check(_lib.load().rexsc_int8_matmul(_ptr(a.data), _ptr(a.scale), _ptr(b.data), _ptr(b.scale), bias_ptr, bias_dtype,
                                              a.rows, b.rows, a.cols, _ptr(out), _DTYPES[dtype], _int8_kernel(), _stream(dev)),
                "rexsc_int8_matmul")
+    if _DEBUG and not torch.cuda.is_current_stream_capturing():
+        _lib.check(int8_status(dev), f"{what} (device status)")
     del keep
     return out
 
@@ -861,12 +863,8 @@ def int8_linear(x: torch.Tensor, weight, bias: torch.Tensor = None) -> torch.Ten
     on the stream of their leaf nodes, which ends the capture, or the process, with an error."""
     host = _lib._host or _lib.host()
     if type(weight) is Int8Matrix:
-        y = host.int8_linear(x, None, weight.data, weight.scale, weight.rows, weight.cols, bias, _int8_kernel())
-    else:
-        y = host.int8_linear(x, weight, None, None, 0, 0, bias, _int8_kernel())
-    if _DEBUG:
-        _lib.check(int8_status(y.device), "int8_linear (device status)")
-    return y
+        return host.int8_linear(x, None, weight.data, weight.scale, weight.rows, weight.cols, bias, _int8_kernel())
+    return host.int8_linear(x, weight, None, None, 0, 0, bias, _int8_kernel())
 
 
 def int8_status(device=None) -> int:
