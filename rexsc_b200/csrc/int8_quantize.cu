@@ -137,7 +137,8 @@ unsigned blocks_for(long long items)
 // g[m, n] = fl32(dy[m, n] col_scale[n]) is quantised by rows, h[m, n] = fl32(dy[m, n] row_scale[m]) by columns: each folds
 // in the scales of the operand whose rows its contraction runs over.  Two passes over dy: in the first every block leaves the
 // largest magnitudes of its rows and columns and their sums, for the bias; the second joins those (no atomics and nothing to
-// clear) and quantises.  Up to about 100 MB of dy the second pass finds it in L2.  8192 x 4096 bf16: 22 and 39 us (67 MB read,
+// clear) and quantises.  The bias's sum is in fp32 along the rows of a warp (32 of them up to 32768 tokens, 512 at the most)
+// and in 64 bits across warps and blocks, so that its error does not grow with the tokens.  Up to about 100 MB of dy the second pass finds it in L2.  8192 x 4096 bf16: 22 and 39 us (67 MB read,
 // 67 MB read and 67 MB written), bound by latency with half the warps an SM could hold: 64 registers a thread; at 48 or 80 the
 // second pass takes 53 and 47 us.  Arithmetic on pairs of values saves instructions here too, and no time.
 constexpr int kGCols = 256;  // columns of a tile of the first pass: a warp has a row of it, eight columns a lane
@@ -213,11 +214,12 @@ grad_amax_kernel(const T *__restrict__ dy, long long m, long long n, long long s
         const long long col = c0 + threadIdx.x;
         const int at = (threadIdx.x & 7) * 32 + (threadIdx.x >> 3);
         if (col < n) {
-            float most = 0.f, sum = 0.f;
+            float most = 0.f;
+            double sum = 0.; // (in fp32 every warp of every block could lose a half step)
 #pragma unroll
             for (int w = 0; w < 8; w++) most = max_nan(most, cmax[w][at]), sum += csum[w][at];
             if (col_most) col_most[(long long)row_block * n + col] = __float_as_uint(most);
-            if (sums) sums[(long long)row_block * n + col] = sum;
+            if (sums) sums[(long long)row_block * n + col] = (float)sum;
         }
     }
     if (row_most) // (behind the last tile's barrier)
@@ -256,7 +258,7 @@ grad_quantize_kernel(const T *__restrict__ dy, long long m, long long n, long lo
     }
     col_s[threadIdx.x] = qg && col < n ? col_scale[col] : 0.f;
     if (db && row_block == 0 && col < n) {
-        float s = 0.f;
+        double s = 0.;
 #pragma unroll 8
         for (int b = 0; b < col_parts; b++) s += sums[(long long)b * n + col];
         db[col] = (B)s;
