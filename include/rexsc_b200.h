@@ -373,6 +373,7 @@ int rexsc_int8_test_waits(int64_t block);
  *                  r' > 0 is not stored as 0.  Blocks with no magnitude of 2^-100 or more are stored as 0.
  *   d_step         int64[2]: steps so far, and a counter that is 0 between calls.  `advance`: this call is the last of a step
  *                  (calls with other parameter types or hyperparameters may precede it on the stream) and adds 1 to it.
+ *   eps            0, or from 2^-126 to 2^126 (smaller ones are no normal numbers in fp32)
  *   d_lr           fp32 on the device in place of `lr`, or null
  *   d_grad_scale, d_found_inf  fp32 as a GradScaler has them, or null; found_inf != 0: nothing is changed, the count neither
  * Everything but d_param, the moments and d_step is only read.  The list may be reused as soon as the call returns.

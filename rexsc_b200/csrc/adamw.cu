@@ -338,7 +338,8 @@ adamw_kernel(const __grid_constant__ AdamLaunch<kList> l)
             }
         };
         // (each operation on the moments is rounded by itself: what is stored in 8 bits is then the same wherever it is
-        //  computed.  The divisor of the weights' change is 0, or neither below 2^-74 nor above 2^84 / sqrt(1 - b2).)
+        //  computed.  The divisor of the weights' change is 0, or not below the smaller of eps, which is a normal number or 0,
+        //  and 2^-74: its approximate reciprocal takes subnormal numbers for 0.)
         if constexpr (!kBits8) {
             float m[8], v[8];
             load8v(a.m + pos, m);
@@ -484,7 +485,7 @@ extern "C" int rexsc_adamw_step(const rexsc_adamw_desc *desc, const rexsc_adamw_
     const bool bits8 = d.state_bits == 8;
     if ((d.state_bits != 8 && d.state_bits != 32) || d.param_dtype < REXSC_F32 || d.param_dtype > REXSC_BF16 ||
         d.grad_dtype < REXSC_F32 || d.grad_dtype > REXSC_BF16 || !(d.beta1 >= 0. && d.beta1 < 1.) ||
-        !(d.beta2 >= 0. && d.beta2 < 1.) || !(d.eps >= 0.) || !(d.weight_decay >= 0.) || (!d.d_lr && !(d.lr >= 0.)) ||
+        !(d.beta2 >= 0. && d.beta2 < 1.) || !(d.eps == 0. || (d.eps >= 0x1p-126 && d.eps < 0x1p126)) || !(d.weight_decay >= 0.) || (!d.d_lr && !(d.lr >= 0.)) ||
         !d.d_exp_avg || !d.d_exp_avg_sq || (bits8 && (!d.d_exp_avg_scale || !d.d_exp_avg_sq_scale)) ||
         ((reinterpret_cast<uintptr_t>(d.d_exp_avg) | reinterpret_cast<uintptr_t>(d.d_exp_avg_sq)) & 31) ||
         (reinterpret_cast<uintptr_t>(d.d_step) & 7))

@@ -199,6 +199,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: betas must lie in [0, 1) (got {b1}, {b2})")
         if not (group["eps"] >= 0 and group["weight_decay"] >= 0):
             raise ValueError("AdamW: eps and weight_decay must not be negative")
+        if group["eps"] and not 2.0 ** -126 <= group["eps"] < 2.0 ** 126:
+            raise ValueError(f"AdamW: eps must be 0 or a normal number in fp32 (got {group['eps']})")
 
     def flat_state(self, group: int = 0) -> Dict[str, torch.Tensor]:
         """The buffers that hold the moments of a parameter group, and its step count: ``exp_avg`` and ``exp_avg_sq`` (fp32),
