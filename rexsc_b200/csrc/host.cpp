@@ -13,6 +13,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
 
@@ -282,6 +283,15 @@ Tensor int8_linear(const Tensor &x, const std::optional<Tensor> &weight_, const 
 }
 
 // ---- AdamW ----------------------------------------------------------------------------------------------------------
+// Pieces of memory [first, second) in rising order
+using Spans = std::vector<std::pair<uintptr_t, uintptr_t>>;
+
+bool touches(const Spans &spans, uintptr_t begin, uintptr_t end)
+{
+    const auto at = std::upper_bound(spans.begin(), spans.end(), begin, [](uintptr_t b, const auto &s) { return b < s.second; });
+    return at != spans.end() && at->first < end; // (the first one that ends behind `begin`)
+}
+
 // What stays of a parameter group between its steps: each parameter's size, strides and place in the flat moment buffers, and
 // those buffers.  Pointers, types, sizes and strides of weights and gradients are looked at anew in every step.
 class AdamWPlan {
@@ -295,6 +305,10 @@ public:
             shapes_.push_back({p.numel(), first, p.strides().vec()});
             first += (p.numel() + 255) / 256;
         }
+        for (size_t i = 0; i < params.size(); i++) by_address_.push_back((uint32_t)i);
+        std::sort(by_address_.begin(), by_address_.end(), [&](uint32_t a, uint32_t b) {
+            return reinterpret_cast<uintptr_t>(params[a].data_ptr()) < reinterpret_cast<uintptr_t>(params[b].data_ptr());
+        });
         d_.state_bits = state_bits;
         d_.d_step = step.data_ptr<int64_t>();
         d_.d_exp_avg = exp_avg.data_ptr();
@@ -313,6 +327,8 @@ public:
         at::NoGradGuard no_grad;
         c10::cuda::CUDAGuard guard(device_);
         std::vector<Tensor> kept, changed;
+        std::vector<int> place(params.size(), -1); // in the table
+        bool lone = true;                          // no gradient shares its storage with any other tensor
         std::vector<rexsc_adamw_tensor> table;
         std::vector<int> kinds;
         table.reserve(params.size());
@@ -335,10 +351,13 @@ public:
                 g = at::empty_strided(p.sizes(), s.strides, g.options().device(device_)).copy_(g);
             table.push_back({p.data_ptr(), g.data_ptr(), s.numel, s.first});
             kinds.push_back(p_code * 4 + code_of(g.scalar_type()));
+            place[i] = (int)table.size() - 1;
+            lone = lone && g.storage().use_count() == 1;
             kept.push_back(std::move(g)); // (until the launch is on the stream)
             changed.push_back(p);
         }
         if (table.empty()) return;
+        keep_apart(table, kinds, place, lone, kept);
         // autograd knows of writes by their versions: a graph that still needs the old weights raises instead of reading new ones
         for (const Tensor &p : changed) torch::autograd::impl::bump_version(p);
         rexsc_adamw_desc d = d_;
@@ -370,6 +389,47 @@ public:
     }
 
 private:
+    // One launch updates all weights at once and reads all gradients: no two weights may hold the same element, and a gradient
+    // that lies in the memory of any of them is read from a copy.  (One with a storage of its own, as a backward pass leaves
+    // it, does not.)
+    void keep_apart(std::vector<rexsc_adamw_tensor> &table, const std::vector<int> &kinds, const std::vector<int> &place, bool lone,
+                    std::vector<Tensor> &grads) const
+    {
+        const auto span = [&](int i) {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(table[i].d_param);
+            return std::make_pair(at, at + (uintptr_t)table[i].numel * (kinds[i] / 4 == REXSC_F32 ? 4 : 2));
+        };
+        // in the order of their memory, unless weights have been given other memory since
+        uintptr_t end = 0;
+        bool ordered = true;
+        for (uint32_t i : by_address_) {
+            if (place[i] < 0) continue;
+            const auto s = span(place[i]);
+            ordered = ordered && s.first >= end;
+            end = s.second;
+        }
+        if (ordered && lone) return;
+        Spans spans;
+        spans.reserve(table.size());
+        for (uint32_t i : by_address_)
+            if (place[i] >= 0) spans.push_back(span(place[i]));
+        if (!ordered) std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); i++)
+            TORCH_CHECK_VALUE(spans[i - 1].second <= spans[i].first, "AdamW: two parameters share memory");
+        const void *apart = nullptr; // a storage that lies apart from all of them: gradients are often pieces of one buffer
+        for (size_t i = 0; i < grads.size(); i++) {
+            const at::Storage &storage = grads[i].storage();
+            if (storage.unsafeGetStorageImpl() == apart) continue;
+            const uintptr_t all = reinterpret_cast<uintptr_t>(storage.data()), at = reinterpret_cast<uintptr_t>(grads[i].data_ptr());
+            if (!touches(spans, all, all + storage.nbytes())) {
+                apart = storage.unsafeGetStorageImpl();
+            } else if (touches(spans, at, at + (uintptr_t)grads[i].numel() * grads[i].element_size())) {
+                grads[i] = grads[i].clone(at::MemoryFormat::Preserve);
+                table[i].d_grad = grads[i].data_ptr();
+            }
+        }
+    }
+
     struct Shape {
         int64_t numel, first;
         std::vector<int64_t> strides;
@@ -377,6 +437,7 @@ private:
     at::Device device_;
     std::vector<Tensor> kept_;
     std::vector<Shape> shapes_;
+    std::vector<uint32_t> by_address_; // the parameters in the order of their memory when the plan was made
     rexsc_adamw_desc d_ = {};
 };
 
