@@ -56,9 +56,13 @@ bool same_places(at::IntArrayRef sizes, at::IntArrayRef a, at::IntArrayRef b)
 
 void *stream_of(const at::Device &d) { return c10::cuda::getCurrentCUDAStream(d.index()).stream(); }
 
+// (views that stand for the negative of what lies in memory, as the imaginary part of a conjugate does, are written out)
+Tensor as_stored(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // t as [rows, cols] whose rows are dense, in a type that the kernels read (a view where that is possible)
-Tensor rows_of(const Tensor &t, int64_t cols)
+Tensor rows_of(const Tensor &given, int64_t cols)
 {
+    const Tensor t = as_stored(given);
     if (t.dim() == 2 && code_of(t.scalar_type()) >= 0 && (t.stride(1) == 1 || cols == 1)) return t;
     Tensor r = code_of(t.scalar_type()) >= 0 ? t : t.to(at::kFloat);
     if (r.dim() != 2) r = r.reshape({-1, cols});
@@ -90,7 +94,7 @@ struct Bias {
         if (!bias.defined()) return;
         TORCH_CHECK_VALUE(bias.device() == d && bias.dim() == 1 && bias.size(0) == n && bias.is_floating_point(),
                           "int8_linear: expected a floating-point bias [", n, "] on ", d);
-        kept = (code_of(bias.scalar_type()) >= 0 ? bias : bias.to(at::kFloat)).contiguous();
+        kept = as_stored(code_of(bias.scalar_type()) >= 0 ? bias : bias.to(at::kFloat)).contiguous();
         ptr = kept.data_ptr();
         dtype = code_of(kept.scalar_type());
     }
@@ -341,12 +345,13 @@ public:
             Tensor g = p.grad();
             if (!g.defined() || s.numel == 0) continue;
             TORCH_CHECK_VALUE(p.layout() == at::kStrided && p.numel() == s.numel && same_places(p.sizes(), p.strides(), s.strides) &&
-                                  p.device() == device_,
+                                  p.device() == device_ && !p.is_neg(),
                               "AdamW: a parameter has changed its size, memory format or device");
             const int p_code = code_of(p.scalar_type());
             TORCH_CHECK_VALUE(p_code >= 0, "AdamW: parameters must be float32, float16 or bfloat16 (got ", p.scalar_type(), ")");
             TORCH_CHECK_VALUE(g.layout() == at::kStrided, "AdamW: sparse gradients are not supported");
             if (code_of(g.scalar_type()) < 0) g = g.to(at::kFloat);
+            g = as_stored(g);
             if (!same_places(p.sizes(), g.strides(), s.strides) || g.sizes() != p.sizes() || g.device() != device_)
                 g = at::empty_strided(p.sizes(), s.strides, g.options().device(device_)).copy_(g);
             table.push_back({p.data_ptr(), g.data_ptr(), s.numel, s.first});
@@ -364,7 +369,7 @@ public:
         const auto scalar = [&](const std::optional<Tensor> &t) -> const float * {
             if (!t) return nullptr;
             TORCH_CHECK_VALUE(t->numel() == 1, "AdamW: expected one element");
-            kept.push_back(t->to(device_, at::kFloat));
+            kept.push_back(as_stored(t->to(device_, at::kFloat)));
             return kept.back().data_ptr<float>();
         };
         d.lr = lr, d.beta1 = beta1, d.beta2 = beta2, d.eps = eps, d.weight_decay = weight_decay;

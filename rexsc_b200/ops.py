@@ -704,7 +704,7 @@ class Int8Matrix:
                 or data.data_ptr() % 256):
             raise ValueError(f"Int8Matrix: expected {nbytes} contiguous bytes of data on 256 for {rows} x {cols}")
         if (scale.device != data.device or scale.dtype != torch.float32 or tuple(scale.shape) != (rows,)
-                or not scale.is_contiguous()):
+                or not scale.is_contiguous() or scale.is_neg() or data.is_neg()):
             raise ValueError(f"Int8Matrix: expected a contiguous float32 scale [{rows}] on {data.device}")
         for name, value in zip(self.__slots__, (rows, cols, data, scale)):
             object.__setattr__(self, name, value)
@@ -740,7 +740,8 @@ class Int8Matrix:
             raise ValueError("Int8Matrix.from_values: expected one scale per row on the values' device")
         dev = values.device
         with _on(dev):
-            v = values if values.stride(1) == 1 or cols == 1 else values.contiguous()
+            v = values.resolve_neg()
+            v = v if v.stride(1) == 1 or cols == 1 else v.contiguous()
             data = _int8_data(rows, cols, dev, "Int8Matrix.from_values")
             _lib.check(_lib.load().rexsc_int8_pack(_ptr(v), rows, cols, v.stride(0), _ptr(data), _stream(dev)),
                        "rexsc_int8_pack")
@@ -771,7 +772,7 @@ def _int8_data(rows: int, cols: int, dev, what: str) -> torch.Tensor:
 
 def _rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
     """``t`` as [rows, cols] whose rows are dense (a view where that is possible)."""
-    t = _float_kind(t.detach())
+    t = _float_kind(t.detach()).resolve_neg()
     if t.dim() != 2:
         t = t.reshape(-1, cols)
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
@@ -806,7 +807,7 @@ def _int8_bias(bias, n: int, dev, what: str):
         return None, 0, 0
     if bias.device != dev or tuple(bias.shape) != (n,) or not bias.is_floating_point():
         raise ValueError(f"{what}: expected a floating-point bias [{n}] on {dev}")
-    bias = _float_kind(bias.detach()).contiguous()
+    bias = _float_kind(bias.detach()).resolve_neg().contiguous()
     return bias, _ptr(bias), _DTYPES[bias.dtype]
 
 

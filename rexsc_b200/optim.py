@@ -144,7 +144,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("AdamW: the parameters of a group must be on one CUDA device")
             if p.dtype not in _DTYPES:
                 raise ValueError(f"AdamW: parameters must be float32, float16 or bfloat16 (got {p.dtype})")
-            if not _dense(p):
+            if not _dense(p) or p.is_neg():
                 raise ValueError("AdamW: parameters must be dense (no gaps or overlaps between their elements)")
         sizes = [p.numel() for p in params]
         blocks = [-(-n // BLOCK) for n in sizes]
