@@ -252,7 +252,7 @@ class AdamW(torch.optim.Optimizer):
             lr = group["lr"]
             group.update({k: copy.deepcopy(v) for k, v in saved.items() if k not in ("params", "param_names", "strides")})
             if isinstance(lr, torch.Tensor):
-                lr.fill_(group["lr"])
+                lr.copy_(torch.as_tensor(group["lr"]).reshape(lr.shape))
                 group["lr"] = lr
         for hook in self._optimizer_load_state_dict_post_hooks.values():
             hook(self)

@@ -103,3 +103,17 @@ def test_names_of_parameters_stay(ops):
     a, b = make("head"), make("tail")
     b.load_state_dict(a.state_dict())
     assert b.param_groups[0]["param_names"] == ["tail"]
+
+
+@pytest.mark.parametrize("mine", [(), (1,), (1, 1)])
+@pytest.mark.parametrize("theirs", [(), (1,), "number", "cpu"])
+def test_shapes_of_a_tensor_lr(ops, mine, theirs):
+    value = 0.25 if theirs == "number" else torch.tensor(0.25) if theirs == "cpu" else torch.full(theirs, 0.25, device="cuda")
+    saved, _ = _make(value)
+    saved.step()
+    lr = torch.full(mine, 1e-3, device="cuda")
+    opt, p = _make(lr)
+    opt.load_state_dict(saved.state_dict())
+    assert opt.param_groups[0]["lr"] is lr and lr.shape == mine and float(lr) == 0.25
+    opt.step()
+    assert int(opt.flat_state()["step"]) == 2
