@@ -216,11 +216,17 @@ class AdamW(torch.optim.Optimizer):
     def state_dict(self):
         """As torch's optimizers give it; the tensors are the optimizer's own.  Moments in 8 bits are stored in the order of
         the weights' memory."""
-        sd = super().state_dict()
-        sd["state"] = {key: dict(views) for key, views in sd["state"].items()}
-        sd["state_bits"] = self._state_bits
-        for i, (strides, plan) in enumerate((p["strides"], p) for p in self._plans):
-            sd["param_groups"][i]["strides"] = [tuple(s) for s in strides]
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
+        number = {p: i for i, p in enumerate(self.state)}
+        groups = [{**group, "params": [number[p] for p in group["params"]], "strides": [tuple(s) for s in plan["strides"]]}
+                  for group, plan in zip(self.param_groups, self._plans)]
+        sd = {"state": {number[p]: dict(views) for p, views in self.state.items()}, "param_groups": groups,
+              "state_bits": self._state_bits}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            changed = hook(self, sd)
+            if changed is not None:
+                sd = changed
         return sd
 
     @torch.no_grad()
