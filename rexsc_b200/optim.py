@@ -46,15 +46,16 @@ class _Views(dict):
 
 
 class _State(Mapping):
-    """All parameters' views of the flat moment buffers, made when they are asked for."""
+    """All parameters' views of the flat moment buffers, made when they are asked for.  (It knows the plans and not the
+    optimizer: the two would keep one another, and the moments, until a garbage collection.)"""
 
-    def __init__(self, place, make):
-        self._place, self._make, self._made = place, make, {}
+    def __init__(self, place):
+        self._place, self._made = place, {}
 
     def __getitem__(self, p) -> _Views:
         made = self._made.get(p)
         if made is None:
-            made = self._made[p] = _Views(self._make(p))
+            made = self._made[p] = _views(*self._place[p])
         return made
 
     def __setitem__(self, p, value) -> None:
@@ -104,7 +105,7 @@ class AdamW(torch.optim.Optimizer):
         self._plans = []
         self._place = {}    # parameter -> (its group's plan, its number there)
         self._built = False
-        self._state = _State(self._place, self._views)
+        self._state = _State(self._place)
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         self._built = True
 
@@ -170,17 +171,6 @@ class AdamW(torch.optim.Optimizer):
                                        flat.get("exp_avg_sqrt_scale"))
         return {"flat": flat, "step": step, "native": native, "first": first, "shapes": [p.shape for p in params],
                 "strides": [p.stride() for p in params]}
-
-    def _views(self, p) -> Dict[str, torch.Tensor]:
-        plan, i = self._place[p]
-        first, last, shape, stride = plan["first"][i], plan["first"][i + 1], plan["shapes"][i], plan["strides"][i]
-        views = {"step": plan["step"][0]}
-        for name, t in plan["flat"].items():
-            if name.endswith("_scale"):
-                views[name] = t[first:last]
-            else:
-                views[name] = t.as_strided(shape, stride, first * BLOCK) if last > first else t[:0].view(shape)
-        return views
 
     def _check_apart(self) -> None:
         """One launch updates all tensors at once: no two of them may hold the same element."""
@@ -293,6 +283,18 @@ class AdamW(torch.optim.Optimizer):
     # torch wraps an optimizer's step in a profiler range and calls the hooks there, 10 us of the host's time in a step
     # whose launch takes 4; the hooks are called above instead
     step.hooked = True
+
+
+def _views(plan: dict, i: int) -> _Views:
+    """Of parameter i of a group's plan."""
+    first, last, shape, stride = plan["first"][i], plan["first"][i + 1], plan["shapes"][i], plan["strides"][i]
+    views = {"step": plan["step"][0]}
+    for name, t in plan["flat"].items():
+        if name.endswith("_scale"):
+            views[name] = t[first:last]
+        else:
+            views[name] = t.as_strided(shape, stride, first * BLOCK) if last > first else t[:0].view(shape)
+    return _Views(views)
 
 
 def _closure_of(optimizer, closure=None):
