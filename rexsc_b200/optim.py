@@ -7,6 +7,7 @@ place in ``utils_own.train``: it is a ``torch.optim.Optimizer``, so learning-rat
 from __future__ import annotations
 
 import copy
+from collections import OrderedDict
 from collections.abc import Mapping
 from typing import Dict
 
@@ -44,6 +45,10 @@ class _Views(dict):
 
     __delitem__ = __ior__ = clear = pop = popitem = setdefault = _refuse
 
+    def __reduce__(self):
+        # copies and pickles are dictionaries of their own, of a kind that torch.load takes as it is
+        return OrderedDict, (), None, None, iter(self.items())
+
 
 class _State(Mapping):
     """All parameters' views of the flat moment buffers, made when they are asked for.  (It knows the plans and not the
@@ -69,6 +74,9 @@ class _State(Mapping):
 
     def __len__(self) -> int:
         return len(self._place)
+
+    def __reduce__(self):
+        return OrderedDict, (), None, None, iter(self.items())
 
 
 BLOCK = 256  # elements of a block of the flat moment buffers (of a scale of 8-bit moments)

@@ -103,3 +103,27 @@ def test_saved_states_hold_plain_dictionaries(ops, bits, tmp_path):
     b.load_state_dict(torch.load(tmp_path / "s.pt", weights_only=True))
     for x, y in zip(opt.flat_state().values(), b.flat_state().values()):
         assert torch.equal(x.view(torch.uint8) if x.dim() else x, y.view(torch.uint8) if y.dim() else y)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_are_dictionaries_of_their_own(ops, bits):
+    import copy
+    import io
+
+    opt, ps = _make(bits)
+    views = opt.state[ps[0]]
+    # (torch.save: plain pickle does not take torch's 8-bit floats)
+    file = io.BytesIO()
+    torch.save(views, file)
+    file.seek(0)
+    for other in (copy.deepcopy(views), torch.load(file, weights_only=True)):
+        assert type(other) is collections.OrderedDict and list(other) == NAMES[bits]
+        for name, t in other.items():
+            assert t.data_ptr() != views[name].data_ptr()
+            assert torch.equal(t.view(torch.uint8) if t.dim() else t, views[name].view(torch.uint8) if t.dim() else views[name])
+            t.zero_()
+    assert type(copy.copy(views)) is collections.OrderedDict and copy.copy(views)["step"] is views["step"]
+    whole = copy.deepcopy(opt.state)
+    assert type(whole) is collections.OrderedDict and len(whole) == 4
+    assert all(type(v) is collections.OrderedDict for v in whole.values())
+    assert int(views["step"]) == 1 and views["exp_avg"].float().abs().sum() > 0
