@@ -847,8 +847,8 @@ def int8_matmul(a: Int8Matrix, b: Int8Matrix, bias: torch.Tensor = None, dtype: 
 def int8_linear(x: torch.Tensor, weight, bias: torch.Tensor = None) -> torch.Tensor:
     """A linear layer in 8-bit integers: ``x`` [..., k] is quantised per token, multiplied with ``weight`` and returned as
     [..., n] in ``x``'s type: float32, float16 or bfloat16.  Any other floating-point type is read as float32, and the output is
-    float32 then; gradients come back in their operands' types.  The plain digital form of the layer that :func:`linear_generic_general_acc` computes on
-    bit streams.
+    float32 then; gradients come back in their operands' types.  The plain digital form of the layer that
+    :func:`linear_generic_general_acc` computes on bit streams.
 
     ``weight``: an :class:`Int8Matrix` [n, k], quantised once per output channel (serving); or a floating-point tensor [n, k]
     that is quantised in the call (training).  Gradients flow to ``x``, to a floating-point ``weight`` and to ``bias``, past

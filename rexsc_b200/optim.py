@@ -87,11 +87,12 @@ class AdamW(torch.optim.Optimizer):
 
         m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps)
 
-    ``params``: dense CUDA tensors in float32, float16 or bfloat16 (others are refused), gradients in any floating-point type.  ``state_bits=32`` keeps m and
-    v in fp32.  ``state_bits=8`` keeps m and sqrt(v) as e4m3 with an fp32 scale for every 256 elements, a sixteenth of a byte
-    per weight beside the two: a quarter of the memory.  Their rounding alternates between the two neighbouring values so that
-    its mean over the steps is right (rounding to nearest would freeze them); it depends on the element's place and the step
-    count alone, so runs repeat.  A gradient that is no finite number spoils its element, with 8 bits its block of 256.
+    ``params``: dense CUDA tensors in float32, float16 or bfloat16 (others are refused), gradients in any floating-point type.
+    ``state_bits=32`` keeps m and v in fp32.  ``state_bits=8`` keeps m and sqrt(v) as e4m3 with an fp32 scale for every 256
+    elements, a sixteenth of a byte per weight beside the two: a quarter of the memory.  Their rounding alternates between the
+    two neighbouring values so that its mean over the steps is right (rounding to nearest would freeze them); it depends on the
+    element's place and the step count alone, so runs repeat.  A gradient that is no finite number spoils its element, with 8
+    bits its block of 256.
 
     ``state`` holds every parameter from the start on; its tensors are views of the buffers (:meth:`flat_state`), and what is
     assigned to them is copied.  An optimizer cannot be copied or pickled: use :meth:`state_dict`.
